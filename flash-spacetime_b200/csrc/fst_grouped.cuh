@@ -1,0 +1,110 @@
+// Grouped-head attention: addressing and the work list shared by its CUDA-core
+// and tensor-core kernels.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "fst_common.cuh"
+#include "fst_internal.h"
+
+namespace fst {
+namespace grouped {
+
+// One block's rows of one event. Rows i0 <= i < min(i0 + BM, lim) belong to
+// the block: those below len are live, the others are rows of no event, whose
+// outputs are written 0.
+struct RowTile {
+  int ev;    // event index of the padded layout, 0 when packed
+  int base;  // buffer row of the event's row 0
+  int len;   // live rows of the event
+  int lim;   // rows the event (or the gap between events) covers
+  int i0;    // first row of the block
+};
+
+// Blocks of bm rows that the work list of `p` needs per head. Packed: event e
+// starts at list position cu[e] / bm + e + 1, which leaves every event at
+// least ceil(len / bm) positions (floor(b) - floor(a) + 1 >= ceil(b - a)), so
+// the list needs no prefix pass and no host synchronisation; the gap before
+// the first event and the one behind the last are entries -1 and B.
+__host__ __device__ __forceinline__ int64_t list_blocks(const FstGroupedProblem& p, int bm) {
+  if (p.packed) return p.total_rows / bm + p.batch + 2;
+  return (int64_t)p.batch * ((p.max_len + bm - 1) / bm);
+}
+
+__device__ __forceinline__ int clamp_row(int x, int64_t n) {
+  return x < 0 ? 0 : (x > n ? (int)n : x);
+}
+// Buffer row at which entry e of the packed list starts (e = -1 .. B + 1).
+// Clamped, so offsets that are wrong never lead out of the tensors.
+__device__ __forceinline__ int entry_row(const FstGroupedProblem& p, int e) {
+  if (e < 0) return 0;
+  if (e > p.batch) return (int)p.total_rows;
+  return clamp_row(__ldg(p.cu_seqlens + e), p.total_rows);
+}
+
+// Entry `id` of the list (called by whole warps). Causal blocks of an event
+// come last rows first (`heavy_last` false) or first rows first, whichever
+// puts the ones with most keys or queries at the front. Returns false when
+// the position is empty.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const FstGroupedProblem& p, int id, bool reverse,
+                                          RowTile& t) {
+  int tile, live;
+  if (!p.packed) {
+    const int per = (p.max_len + BM - 1) / BM;
+    t.ev = id / per;
+    tile = id - t.ev * per;
+    t.base = 0;
+    t.len = clamp_row(__ldg(p.seqlens + t.ev), p.max_len);
+    t.lim = p.max_len;
+  } else {
+    // Largest entry whose position is <= id: 33-way search, one probe a lane.
+    const int lane = threadIdx.x & 31;
+    int lo = -1, hi = p.batch + 1;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 32) / 33;
+      const int e = lo + step * (lane + 1);
+      const bool at = e < hi && entry_row(p, e) / BM + e + 1 <= id;
+      const int n = __ffs(~__ballot_sync(0xffffffffu, at)) - 1;  // -1 + 1 .. 32
+      const int steps = n < 0 ? 32 : n;
+      lo += step * steps;
+      hi = min(hi, lo + step);
+    }
+    const int a = entry_row(p, lo), b = entry_row(p, lo + 1);
+    t.ev = 0;
+    t.base = a;
+    t.lim = max(b - a, 0);
+    t.len = (lo >= 0 && lo < p.batch) ? t.lim : 0;
+    tile = id - (a / BM + lo + 1);
+  }
+  live = (t.len + BM - 1) / BM;
+  if (reverse && tile < live) tile = live - 1 - tile;
+  // A position behind the entry's last block is empty (and tile * BM stays
+  // far below 2^31: tile <= list_blocks <= 2^31 / BM + B + 2 only for BM >= 64
+  // and rows < 2^31, so compare before multiplying).
+  if (tile >= (t.lim + BM - 1) / BM) return false;
+  t.i0 = tile * BM;
+  return true;
+}
+
+template <typename T>
+__device__ __forceinline__ T* row_ptr(const FstRows& r, const RowTile& t, int h, int i) {
+  return (T*)r.data + (int64_t)t.ev * r.event_stride + (int64_t)h * r.head_stride +
+         (int64_t)(t.base + i) * r.row_stride;
+}
+
+// Offset of (h, row t.base + i) in a dense statistics tensor of nh heads.
+__device__ __forceinline__ int64_t stat_at(const FstGroupedProblem& p, const RowTile& t, int nh,
+                                           int h, int i) {
+  const int64_t n = p.packed ? p.total_rows : p.max_len;
+  return ((int64_t)t.ev * nh + h) * n + t.base + i;
+}
+
+// Host side (fst_grouped_simt.cu, fst_grouped_fwd.cu, fst_grouped_bwd.cu).
+int simt_forward(const FstGroupedForwardArgs& a, cudaStream_t st);
+int simt_backward(const FstGroupedBackwardArgs& a, cudaStream_t st);
+
+}  // namespace grouped
+}  // namespace fst

@@ -21,6 +21,8 @@ int allow_dynamic_smem(const void* fn, int bytes, std::atomic<uint64_t>& done);
 // of ncw dW and ncb db columns in a fixed order (NULL outputs skipped).
 int launch_sum_partials(const float* dw_partial, const float* db_partial, int64_t rows, int ncw,
                         int ncb, float* dw, float* db, cudaStream_t st);
+// fst_rotary after validation.
+int launch_rotary(const FstRotaryArgs& p, cudaStream_t st);
 namespace simt {
 int launch_fwd(const FstForwardArgs& a, cudaStream_t st);
 int launch_bwd(const FstBackwardArgs& a, cudaStream_t st);

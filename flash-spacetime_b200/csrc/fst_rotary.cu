@@ -1,0 +1,235 @@
+// Rotary positions: rotates the first 2 * pairs channels of every row of q and
+// k by position * freqs[pair], in one launch.
+//
+// One read and one write of every element is all it moves, so HBM is the
+// bound; the rest is arranged around that. A block takes a few rows (about
+// four 32-byte slots per thread) with all their heads, so the angles are
+// formed once per row and pair and shared by the heads through shared memory;
+// each thread issues its loads before the angles are formed.
+//
+// The angle is position * freq, which for far positions reaches 1e6 rad and
+// more: fp32 would lose its phase. It is taken in turns in fp64,
+// t = position * (freq / 2 pi), reduced exactly by t - rint(t), and only the
+// remainder (at most half a turn) is rounded to fp32 for sincospif: 2^-25
+// turns, 2e-7 rad, whatever the position.
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "fst_common.cuh"
+#include "fst_internal.h"
+
+namespace fst {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kItems = 4;         // slots per thread and pass
+constexpr int kMaxRows = 16;      // rows per block
+constexpr int kMaxTable = 2048;   // (cos, sin) pairs in shared memory
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T x[V];
+};
+
+// A slot is two vectors of V channels, `a` and `b`: in a rotated slot of the
+// half layout the two halves of V pairs; else 2 V consecutive channels (b may
+// fall behind the head's end).
+struct Slot {
+  int a, b;      // first channels
+  int pair;      // first pair, or -1: copied
+  bool has_b;
+};
+
+template <int V>
+__device__ __forceinline__ Slot slot_at(const FstRotaryArgs& p, int s) {
+  Slot t;
+  const int rotated = p.interleaved ? (2 * p.pairs + 2 * V - 1) / (2 * V) : p.pairs / V;
+  if (!p.interleaved && s < rotated) {
+    t.a = s * V;
+    t.b = p.pairs + s * V;
+    t.pair = s * V;
+  } else {
+    t.a = p.interleaved ? s * 2 * V : 2 * p.pairs + (s - rotated) * 2 * V;
+    t.b = t.a + V;
+    t.pair = s < rotated ? t.a / 2 : -1;
+  }
+  t.has_b = t.b < p.head_dim;
+  return t;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void rotate(const FstRotaryArgs& p, const Slot& t, const float2* cs,
+                                       Vec<T, V>& a, Vec<T, V>& b) {
+  if (t.pair < 0) return;
+  if (!p.interleaved || V == 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float2 c = cs[t.pair + e];
+      const float x = to_f<T>(a.x[e]), y = to_f<T>(b.x[e]);
+      a.x[e] = from_f<T>(x * c.x - y * c.y);
+      b.x[e] = from_f<T>(y * c.x + x * c.y);
+    }
+  } else {
+    // Pairs lie inside the vectors; the slot may reach past the rotated part.
+#pragma unroll
+    for (int e = 0; e + 1 < V; e += 2) {
+      const int pa = t.pair + e / 2, pb = pa + V / 2;
+      if (pa < p.pairs) {
+        const float2 c = cs[pa];
+        const float x = to_f<T>(a.x[e]), y = to_f<T>(a.x[e + 1]);
+        a.x[e] = from_f<T>(x * c.x - y * c.y);
+        a.x[e + 1] = from_f<T>(y * c.x + x * c.y);
+      }
+      if (pb < p.pairs) {
+        const float2 c = cs[pb];
+        const float x = to_f<T>(b.x[e]), y = to_f<T>(b.x[e + 1]);
+        b.x[e] = from_f<T>(x * c.x - y * c.y);
+        b.x[e + 1] = from_f<T>(y * c.x + x * c.y);
+      }
+    }
+  }
+}
+
+// Position of flat row `row` ((ev, i) when padded); false: a packed row of no
+// event.
+__device__ __forceinline__ bool position_of(const FstRotaryArgs& p, int64_t row, int64_t i,
+                                            int64_t& pos) {
+  if (p.positions) {
+    pos = p.positions_64 ? ((const int64_t*)p.positions)[row] : ((const int32_t*)p.positions)[row];
+    return true;
+  }
+  pos = i;
+  if (!p.packed) return true;
+  if (p.batch <= 0 || row < p.cu_seqlens[0] || row >= p.cu_seqlens[p.batch]) return false;
+  int lo = 0, hi = p.batch;  // cu[lo] <= row < cu[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cu_seqlens[mid] <= row)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  pos = row - p.cu_seqlens[lo];
+  return true;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(FstRotaryArgs p, int rows_per_block,
+                                                          int slots) {
+  __shared__ float2 cs[kMaxTable];
+  __shared__ double pos[kMaxRows];
+  __shared__ int live[kMaxRows];
+  __shared__ int64_t offs[kMaxRows][4];  // element offset of the row: q, q_out, k, k_out
+  const int64_t row0 = (int64_t)blockIdx.x * rows_per_block;
+  const int rows = (int)min((int64_t)rows_per_block, p.total_rows - row0);
+  const int heads = p.heads + (p.k.data ? p.kv_heads : 0);
+  if (threadIdx.x < rows) {
+    const int64_t row = row0 + threadIdx.x;
+    const int64_t ev = p.packed ? 0 : row / p.max_len;
+    const int64_t i = p.packed ? row : row - ev * p.max_len;
+    int64_t at = 0;
+    live[threadIdx.x] = position_of(p, row, i, at);
+    pos[threadIdx.x] = (double)at;
+    offs[threadIdx.x][0] = ev * p.q.event_stride + i * p.q.row_stride;
+    offs[threadIdx.x][1] = ev * p.q_out.event_stride + i * p.q_out.row_stride;
+    offs[threadIdx.x][2] = ev * p.k.event_stride + i * p.k.row_stride;
+    offs[threadIdx.x][3] = ev * p.k_out.event_stride + i * p.k_out.row_stride;
+  }
+  __syncthreads();
+  using W = Vec<T, V>;
+  const int items = rows * heads * slots;  // host: below 2^31
+  for (int base = 0; base < items; base += kThreads * kItems) {
+    W a[kItems], b[kItems];
+    T* dst[kItems];
+    Slot slot[kItems];
+    int row[kItems];
+#pragma unroll
+    for (int n = 0; n < kItems; ++n) {
+      const int item = base + n * kThreads + threadIdx.x;
+      dst[n] = nullptr;
+      if (item >= items) continue;
+      const int s = item % slots, rh = item / slots;
+      const int h = rh % heads, r = rh / heads;
+      row[n] = r;
+      slot[n] = slot_at<V>(p, s);
+      const bool is_k = h >= p.heads;
+      const FstRows& in = is_k ? p.k : p.q;
+      const FstRows& out = is_k ? p.k_out : p.q_out;
+      const int hh = is_k ? h - p.heads : h;
+      const T* src = (const T*)in.data + offs[r][is_k ? 2 : 0] + hh * in.head_stride;
+      dst[n] = (T*)out.data + offs[r][is_k ? 3 : 1] + hh * out.head_stride;
+      a[n] = *(const W*)(src + slot[n].a);
+      if (slot[n].has_b) b[n] = *(const W*)(src + slot[n].b);
+    }
+    if (base == 0) {
+      for (int e = threadIdx.x; e < rows * p.pairs; e += kThreads) {
+        const int r = e / p.pairs;
+        float sn = 0.f, c = 1.f;
+        if (live[r]) {
+          const double t = pos[r] * (p.freqs[e - r * p.pairs] * 0.15915494309189533577);
+          sincospif((float)(2.0 * (t - rint(t))), &sn, &c);
+          sn *= p.inverse ? -p.magnitude : p.magnitude;
+          c *= p.magnitude;
+        }
+        cs[e] = make_float2(c, sn);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < kItems; ++n) {
+      if (!dst[n]) continue;
+      rotate<T, V>(p, slot[n], cs + row[n] * p.pairs, a[n], b[n]);
+      *(W*)(dst[n] + slot[n].a) = a[n];
+      if (slot[n].has_b) *(W*)(dst[n] + slot[n].b) = b[n];
+    }
+  }
+}
+
+bool vector_ok(const FstRows& r, int v) {
+  return ((uintptr_t)r.data & 15) == 0 && r.event_stride % v == 0 && r.head_stride % v == 0 &&
+         r.row_stride % v == 0;
+}
+
+template <typename T>
+int launch(const FstRotaryArgs& p, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  // 16-byte vectors where every row starts on 16 bytes and neither the head
+  // nor (half layout) its rotated halves end inside a vector; else elements.
+  const bool vec = p.head_dim % V == 0 && (p.interleaved || p.pairs % V == 0) &&
+                   vector_ok(p.q, V) && vector_ok(p.q_out, V) &&
+                   (!p.k.data || (vector_ok(p.k, V) && vector_ok(p.k_out, V)));
+  const int w = vec ? V : 1;
+  const int rot = p.interleaved ? (2 * p.pairs + 2 * w - 1) / (2 * w) : p.pairs / w;
+  const int slots = p.interleaved ? (p.head_dim + 2 * w - 1) / (2 * w)
+                                  : rot + (p.head_dim - 2 * p.pairs + 2 * w - 1) / (2 * w);
+  const int64_t row_items = (int64_t)(p.heads + (p.k.data ? p.kv_heads : 0)) * slots;
+  if (row_items * kMaxRows >= (1ll << 31))
+    return api_fail(FST_ERR_UNSUPPORTED, "rotary: %d heads of %d are too many", p.heads,
+                    p.head_dim);
+  int64_t rows = kThreads * kItems / row_items;
+  if (rows > kMaxRows) rows = kMaxRows;
+  if (p.pairs > 0 && rows > kMaxTable / p.pairs) rows = kMaxTable / p.pairs;
+  if (rows < 1) rows = 1;
+  const int64_t blocks = (p.total_rows + rows - 1) / rows;
+  if (blocks >= (1ll << 31))
+    return api_fail(FST_ERR_UNSUPPORTED, "rotary: %lld rows are too many",
+                    (long long)p.total_rows);
+  if (vec)
+    rotary_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(p, (int)rows, slots);
+  else
+    rotary_kernel<T, 1><<<(unsigned)blocks, kThreads, 0, st>>>(p, (int)rows, slots);
+  count_launch();
+  return FST_OK;
+}
+
+}  // namespace
+
+int launch_rotary(const FstRotaryArgs& p, cudaStream_t st) {
+  if (p.dtype == FST_F32) return launch<float>(p, st);
+  if (p.dtype == FST_BF16) return launch<__nv_bfloat16>(p, st);
+  return launch<__half>(p, st);
+}
+
+}  // namespace fst

@@ -14,6 +14,11 @@ The exported names are those of the upstream ``flash_spacetime`` package
 (upstream src/flash_spacetime/__init__.py:38-54). ``reference`` holds the
 pure-PyTorch definition and is importable without a GPU; the fused entry
 points load the CUDA library on first use.
+
+Beside the spacetime ops stand those that a model's other blocks need:
+``flash_grouped_attention`` / ``flash_grouped_attention_varlen`` (no pair
+term, fewer key than query heads, causal or not) and ``flash_rotary`` /
+``flash_rotary_varlen`` (positions by rotation).
 """
 
 from .reference import (  # noqa: F401
@@ -23,8 +28,12 @@ from .reference import (  # noqa: F401
     TIME_SCALE,
     attention_rel_oracle_inputs,
     float_padding_mask,
+    grouped_attention_reference,
     merge_heads,
     pair_mask_bias,
+    rotary_frequencies,
+    rotary_magnitude,
+    rotary_reference,
     sinusoidal_frequencies,
     spacetime_attention_reference,
     spacetime_pair_features,
@@ -60,4 +69,12 @@ def __getattr__(name: str) -> object:
         from . import ops
 
         return getattr(ops, name)
+    if name in ("flash_grouped_attention", "flash_grouped_attention_varlen"):
+        from . import grouped
+
+        return getattr(grouped, name)
+    if name in ("flash_rotary", "flash_rotary_varlen"):
+        from . import rotary
+
+        return getattr(rotary, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

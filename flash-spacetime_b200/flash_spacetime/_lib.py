@@ -21,7 +21,7 @@ FST_ERR_CUDA = 3
 FST_ERR_WORKSPACE = 4
 FST_ERR_DEVICE = 5
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 FST_FLAG_SHARE_SMS = 1  # FstProblem.flags: another kernel shares the SMs
 FST_FLAG_LONGEST_FIRST = 2  # FstProblem.flags: the library orders the events itself
 MAX_SELF_ORDERED = 1024  # events FST_FLAG_LONGEST_FIRST accepts
@@ -36,6 +36,9 @@ EXPORTED = (
     "fst_backward",
     "fst_forward_noalloc",
     "fst_upload_rows",
+    "fst_grouped_forward",
+    "fst_grouped_backward",
+    "fst_rotary",
     "fst_kernel_launches",
     "fst_last_error",
 )
@@ -106,6 +109,85 @@ class FstBackwardArgs(ctypes.Structure):
     ]
 
 
+class FstRows(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("event_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+    ]
+
+
+class FstGroupedProblem(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("packed", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("total_rows", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("flags", ctypes.c_int32),
+        ("seqlens", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+    ]
+
+
+class FstGroupedForwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("prob", FstGroupedProblem),
+        ("q", FstRows),
+        ("k", FstRows),
+        ("v", FstRows),
+        ("out", FstRows),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
+class FstGroupedBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("prob", FstGroupedProblem),
+        ("q", FstRows),
+        ("k", FstRows),
+        ("v", FstRows),
+        ("out", FstRows),
+        ("dout", FstRows),
+        ("dq", FstRows),
+        ("dk", FstRows),
+        ("dv", FstRows),
+        ("lse", ctypes.c_void_p),
+        ("delta", ctypes.c_void_p),
+    ]
+
+
+class FstRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("packed", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("pairs", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("positions_64", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+        ("total_rows", ctypes.c_int64),
+        ("freqs", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("q", FstRows),
+        ("k", FstRows),
+        ("q_out", FstRows),
+        ("k_out", FstRows),
+    ]
+
+
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
 
@@ -145,6 +227,13 @@ def load() -> ctypes.CDLL:
         lib.fst_upload_rows.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                         ctypes.c_int64, ctypes.c_void_p]
+        lib.fst_grouped_forward.restype = ctypes.c_int
+        lib.fst_grouped_forward.argtypes = [ctypes.POINTER(FstGroupedForwardArgs), ctypes.c_void_p]
+        lib.fst_grouped_backward.restype = ctypes.c_int
+        lib.fst_grouped_backward.argtypes = [ctypes.POINTER(FstGroupedBackwardArgs),
+                                             ctypes.c_void_p]
+        lib.fst_rotary.restype = ctypes.c_int
+        lib.fst_rotary.argtypes = [ctypes.POINTER(FstRotaryArgs), ctypes.c_void_p]
         lib.fst_kernel_launches.restype = ctypes.c_int64
         lib.fst_last_error.restype = ctypes.c_int
         lib.fst_last_error.argtypes = [ctypes.c_char_p, ctypes.c_size_t]

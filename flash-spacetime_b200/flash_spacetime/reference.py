@@ -23,6 +23,7 @@ upstream frequency ladder already does (reference.py:82). With ``C == Dh`` the
 two definitions are the same computation.
 """
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -179,3 +180,104 @@ def attention_rel_oracle_inputs(
     v = lin(src, attention.proj_v.weight, attention.v_bias)
     h = attention.num_heads
     return split_heads(q, h), split_heads(k, h), split_heads(v, h)
+
+
+def grouped_attention_reference(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    seqlens: Optional[Tensor] = None,
+    scale: Optional[float] = None,
+    causal: bool = True,
+) -> Tensor:
+    """Eager definition of grouped-head attention (no upstream counterpart).
+
+    q ``[B, H, L, Dh]``, k and v ``[B, Hkv, L, Dh]``; rows at or past
+    ``seqlens[b]`` are padding: not read, and 0 in the result.
+    """
+    batch, heads, length, dim = q.shape
+    group = heads // k.shape[1]
+    pos = torch.arange(length, device=q.device)
+    if seqlens is None:
+        seqlens = torch.full((batch,), length, device=q.device)
+    valid = valid_row_mask(batch, length, seqlens)[:, None, :, None]
+    q, k, v = (t.masked_fill(~valid, 0) for t in (q, k, v))
+    k, v = (t.repeat_interleave(group, dim=1) for t in (k, v))
+    seen = valid & valid.transpose(2, 3)
+    if causal:
+        seen = seen & (pos[None, :] <= pos[:, None])
+    logits = (q @ k.transpose(-2, -1)) * (dim**-0.5 if scale is None else scale)
+    logits = logits.masked_fill(~seen, float("-inf")).masked_fill(~valid, 0)
+    return (logits.softmax(-1) @ v).masked_fill(~valid, 0)
+
+
+def rotary_frequencies(
+    rotary_dim: int,
+    base: float = 10000.0,
+    *,
+    scaling: Optional[str] = None,
+    factor: float = 1.0,
+    trained_len: int = 4096,
+    fast_turns: float = 32.0,
+    slow_turns: float = 1.0,
+) -> Tensor:
+    """float64 ``[R/2]`` angles per position for ``flash_rotary``.
+
+    ``base ** (-2 p / R)`` for pair p of ``rotary_dim`` = R channels, scaled
+    for contexts ``factor`` times longer than the ``trained_len`` positions:
+
+    * ``"linear"``: every frequency divided by the factor;
+    * ``"base"``: the base times ``factor ** (R / (R - 2))``, which divides the
+      slowest frequency by the factor and leaves the fastest;
+    * ``"parts"``: pairs that turn ``fast_turns`` times or more over
+      ``trained_len`` keep their frequency, those that turn ``slow_turns``
+      times or less are divided by the factor, a ramp linear in the turns
+      between (used with ``rotary_magnitude(factor)``).
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim (={rotary_dim}) must be even and at least 2")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError(f"scaling must be 'linear', 'base', 'parts' or None, got {scaling!r}")
+    if not factor > 0:
+        raise ValueError(f"factor must be positive, got {factor}")
+    if scaling == "base" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    half = rotary_dim // 2
+    freqs = float(base) ** (-torch.arange(half, dtype=torch.float64) / half)
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "parts":
+        if not fast_turns > slow_turns:
+            raise ValueError("fast_turns must exceed slow_turns")
+        turns = trained_len * freqs / (2 * math.pi)
+        keep = ((turns - slow_turns) / (fast_turns - slow_turns)).clamp(0.0, 1.0)
+        freqs = freqs * keep + freqs / factor * (1.0 - keep)
+    return freqs
+
+
+def rotary_magnitude(factor: float) -> float:
+    """Magnitude that goes with ``"parts"`` scaling: ``0.1 ln(factor) + 1``
+    (1 for factors up to 1)."""
+    return 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+
+
+def rotary_reference(
+    x: Tensor,
+    freqs: Tensor,
+    positions: Tensor,
+    interleaved: bool = False,
+    magnitude: float = 1.0,
+) -> Tensor:
+    """Eager definition of the rotation, in float64, rounded once to x's dtype.
+
+    ``x`` is ``[..., Dh]``; ``positions`` broadcasts against ``x[..., 0]``.
+    """
+    angle = positions.double().unsqueeze(-1) * freqs.to(x.device, torch.float64)
+    cos, sin = magnitude * torch.cos(angle), magnitude * torch.sin(angle)
+    rot = 2 * freqs.numel()
+    y = x.double()
+    head = y[..., :rot]
+    a, b = (head[..., 0::2], head[..., 1::2]) if interleaved else head.chunk(2, -1)
+    lo, hi = a * cos - b * sin, b * cos + a * sin
+    head = torch.stack((lo, hi), -1).flatten(-2) if interleaved else torch.cat((lo, hi), -1)
+    return torch.cat((head, y[..., rot:]), -1).to(x.dtype)

@@ -1,0 +1,170 @@
+"""Rotary positions for q and k, before an attention op of this package.
+
+``flash_rotary`` (padded) and ``flash_rotary_varlen`` (packed) rotate the
+channel pairs of q and k by ``position * freqs`` in one launch of
+``fst_rotary``; ``reference.rotary_frequencies`` makes the frequencies. The
+gradient is the rotation by the opposite angle, so nothing of q and k is kept
+for the backward.
+"""
+
+import ctypes
+from typing import Any, Optional, Tuple
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .grouped import _check_tensor, _integers, _rows, _shape
+from .ops import _DTYPES, _ptr, _stream, _timed_call
+
+
+def _adjacent(t: Tensor) -> Tensor:
+    """``t``, copied if a head's channels are not adjacent."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _rotate(q: Tensor, k: Optional[Tensor], layout: str, freqs: Tensor, cu: Optional[Tensor],
+            positions: Optional[Tensor], interleaved: bool, magnitude: float,
+            inverse: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        q = _adjacent(q)
+        k = None if k is None else _adjacent(k)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        events, rows, heads, dim = _shape(q, layout, "q")
+        a = _lib.FstRotaryArgs()
+        a.dtype, a.packed, a.heads, a.head_dim = _DTYPES[q.dtype], int(layout == "packed"), heads, dim
+        a.kv_heads = 0 if k is None else _shape(k, layout, "k")[2]
+        if a.packed:
+            a.batch, a.total_rows = (0 if cu is None else cu.numel() - 1), rows
+        else:
+            a.batch, a.max_len, a.total_rows = events, rows, events * rows
+        a.pairs, a.interleaved, a.inverse = freqs.numel(), int(interleaved), int(inverse)
+        a.magnitude = magnitude
+        a.freqs, a.cu_seqlens, a.positions = _ptr(freqs), _ptr(cu), _ptr(positions)
+        a.positions_64 = int(positions is not None and positions.dtype == torch.int64)
+        a.q, a.k = _rows(q, layout), _rows(k, layout)
+        a.q_out, a.k_out = _rows(q_out, layout), _rows(k_out, layout)
+        rc = _timed_call("fst_rotary", lib.fst_rotary, (ctypes.byref(a), _stream(q.device)),
+                         q.device)
+    _lib.check(rc, "fst_rotary")
+    return q_out, k_out
+
+
+class _FlashRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
+                positions: Optional[Tensor], layout: str, interleaved: bool,
+                magnitude: float) -> Tuple[Tensor, Optional[Tensor]]:  # type: ignore[override]
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(freqs, cu, positions)
+        ctx.how = (layout, interleaved, magnitude)
+        return _rotate(q, k, layout, freqs, cu, positions, interleaved, magnitude, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, gq: Optional[Tensor], gk: Optional[Tensor]):  # type: ignore[override]
+        freqs, cu, positions = ctx.saved_tensors
+        layout, interleaved, magnitude = ctx.how
+        gq = gq if ctx.needs_input_grad[0] else None
+        gk = gk if ctx.needs_input_grad[1] else None
+        dq = dk = None
+        if gq is not None:
+            dq, dk = _rotate(gq, gk, layout, freqs, cu, positions, interleaved, magnitude, True)
+        elif gk is not None:
+            dk, _ = _rotate(gk, None, layout, freqs, cu, positions, interleaved, magnitude, True)
+        return dq, dk, None, None, None, None, None, None
+
+
+def _apply(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
+           positions: Optional[Tensor], layout: str, interleaved: bool,
+           magnitude: float) -> Tuple[Tensor, Optional[Tensor]]:
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {q.dtype}")
+    events, rows, heads, dim = _shape(q, layout, "q")
+    _check_tensor(q, q, "q")
+    if k is not None:
+        _check_tensor(k, q, "k")
+        if _shape(k, layout, "k")[:2] != (events, rows) or k.shape[-1] != dim:
+            raise ValueError(f"k {tuple(k.shape)} must have q's events, rows and Dh, q is "
+                             f"{tuple(q.shape)}")
+        if _shape(k, layout, "k")[2] < 1:
+            raise ValueError("k has no heads (pass k=None)")
+    if heads < 1 or not 1 <= dim <= 1024:
+        raise ValueError(f"q must have heads of 1 to 1024 channels, got {tuple(q.shape)}")
+    if freqs.dim() != 1 or not freqs.dtype.is_floating_point or 2 * freqs.numel() > dim:
+        raise ValueError(f"freqs must be [R/2] floats with R <= Dh (={dim}), got "
+                         f"{tuple(freqs.shape)} {freqs.dtype}")
+    if freqs.requires_grad:
+        raise ValueError("freqs must not require grad")
+    freqs = freqs.to(device=q.device, dtype=torch.float64).contiguous()
+    if positions is not None:
+        _integers(positions, "positions")
+        want = (rows,) if layout == "packed" else (events, rows)
+        if layout != "packed" and positions.shape == (rows,):
+            positions = positions.expand(want)
+        if tuple(positions.shape) != want:
+            raise ValueError(f"positions must be {list(want)}, got {list(positions.shape)}")
+        if positions.dtype not in (torch.int32, torch.int64):
+            positions = positions.to(torch.int32)
+        positions = positions.to(q.device).contiguous()
+    return _FlashRotary.apply(q, k, freqs, cu, positions, layout, bool(interleaved),
+                              float(magnitude))
+
+
+def flash_rotary(
+    q: Tensor,
+    k: Optional[Tensor],
+    freqs: Tensor,
+    positions: Optional[Tensor] = None,
+    *,
+    layout: str = "bhld",
+    interleaved: bool = False,
+    magnitude: float = 1.0,
+) -> Tuple[Tensor, Optional[Tensor]]:
+    """Rotate q and k of a padded batch by their positions.
+
+    q: ``[B, H, L, Dh]``, k: ``[B, Hkv, L, Dh]`` or None (``[B, L, heads, Dh]``
+    with ``layout='blhd'``; fp32, bf16 or fp16, Dh up to 1024). ``freqs``:
+    ``[R/2]`` radians per position for the first R <= Dh channels; the others
+    are copied. Channels p and p + R/2 form pair p, or 2p and 2p + 1 when
+    ``interleaved``. ``positions``: ``[B, L]`` or ``[L]`` integers, by default
+    the row's index; the angle is formed in float64, so any position keeps its
+    phase. ``magnitude`` multiplies the rotated channels
+    (``rotary_magnitude``). Returns new ``(q, k)`` of the same shapes; every
+    row is rotated, padding rows too. Differentiable once in q and k.
+    """
+    if layout not in ("bhld", "blhd"):
+        raise ValueError(f"layout must be 'bhld' or 'blhd', got {layout!r}")
+    return _apply(q, k, freqs, None, positions, layout, interleaved, magnitude)
+
+
+def flash_rotary_varlen(
+    q: Tensor,
+    k: Optional[Tensor],
+    freqs: Tensor,
+    cu_seqlens: Optional[Tensor] = None,
+    positions: Optional[Tensor] = None,
+    *,
+    interleaved: bool = False,
+    magnitude: float = 1.0,
+) -> Tuple[Tensor, Optional[Tensor]]:
+    """Rotate packed q ``[T, H, Dh]`` and k ``[T, Hkv, Dh]`` (or None).
+
+    A row's position is its index in its event (``cu_seqlens``, ``[B+1]``
+    ascending offsets; rows of no event are copied unrotated), or
+    ``positions`` ``[T]`` when given. The rest as for :func:`flash_rotary`.
+    """
+    cu = None
+    if positions is None:
+        if cu_seqlens is None:
+            raise ValueError("pass cu_seqlens or positions")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError("cu_seqlens must be a [B+1] tensor")
+        cu = _integers(cu_seqlens, "cu_seqlens")
+        if cu.dtype == torch.int64:
+            cu = cu.clamp(0, 2**31 - 1)
+        cu = cu.to(device=q.device, dtype=torch.int32).contiguous()
+    return _apply(q, k, freqs, cu, positions, "packed", interleaved, magnitude)

@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define FST_ABI_VERSION 5
+#define FST_ABI_VERSION 6
 
 /* Storage dtype of q, k, v, u, wt, out, dout, dq, dk, dv. */
 enum FstDtype { FST_F32 = 0, FST_BF16 = 1, FST_F16 = 2 };
@@ -227,6 +227,115 @@ int fst_forward_noalloc(const FstForwardArgs* args, void* stream);
  * groups = 1 and row_bytes = fs * 4. */
 int fst_upload_rows(void* dst, const void* src, const int32_t* lens, int64_t batch,
                     int64_t groups, int64_t max_len, int64_t row_bytes, void* stream);
+
+/* ---- grouped-head attention (no upstream counterpart) ----------------------
+ *
+ * The same attention without the pair term, for the blocks of a model that
+ * have none:
+ *
+ *   s_ij  = scale * q_i . k_j   (j <= i when causal)
+ *   P     = softmax_j(s);  out_i = sum_j P_ij v_j;  lse_i = log sum_j exp(s_ij)
+ *
+ * where query head h reads key / value head h / (heads / kv_heads), over
+ * events laid out as for fst_forward. Every tensor is given by a base pointer
+ * and its strides, so the padded [B, H, L, Dh] and [B, L, H, Dh], the packed
+ * [T, H, Dh] and views into a fused projection are all read and written in
+ * place.
+ */
+
+/* A [event, head, row, Dh] tensor: element (b, h, i, d) is data[b * event_stride
+ * + h * head_stride + i * row_stride + d]; strides in elements. Packed
+ * tensors ignore event_stride (row i is the row in the whole buffer). */
+typedef struct FstRows {
+  void* data;
+  int64_t event_stride;
+  int64_t head_stride;
+  int64_t row_stride;
+} FstRows;
+
+typedef struct FstGroupedProblem {
+  int32_t dtype;          /* enum FstDtype                                   */
+  int32_t packed;         /* 0 padded (seqlens), 1 packed (cu_seqlens)       */
+  int32_t batch;          /* B: number of events                             */
+  int32_t heads;          /* H query heads                                   */
+  int32_t kv_heads;       /* Hkv key / value heads; divides H                */
+  int32_t max_len;        /* padded: L. packed: ignored                      */
+  int32_t head_dim;       /* Dh, 1 to 128                                    */
+  int32_t causal;         /* row i sees keys j <= i of its event             */
+  int64_t total_rows;     /* padded: B*L. packed: T. Below 2^31              */
+  float scale;            /* logit scale, finite                             */
+  int32_t flags;          /* 0                                               */
+  const int32_t* seqlens;    /* [B] device, valid prefix lengths (padded)     */
+  const int32_t* cu_seqlens; /* [B+1] device row offsets (packed)             */
+} FstGroupedProblem;
+
+/* Per-row statistics (lse, delta) are dense fp32 [B, H, L] (padded) or [H, T]
+ * (packed). Rows of no event -- padding, or packed rows outside
+ * [cu_seqlens[0], cu_seqlens[B]) -- are never read and are written 0 in out,
+ * dq, dk and dv; their lse and delta are left as they were. */
+typedef struct FstGroupedForwardArgs {
+  FstGroupedProblem prob;
+  FstRows q;             /* H heads                                          */
+  FstRows k;             /* Hkv heads                                        */
+  FstRows v;
+  FstRows out;           /* output, H heads                                  */
+  float* lse;            /* output                                           */
+} FstGroupedForwardArgs;
+
+typedef struct FstGroupedBackwardArgs {
+  FstGroupedProblem prob;
+  FstRows q;
+  FstRows k;
+  FstRows v;
+  FstRows out;           /* forward output                                   */
+  FstRows dout;          /* its gradient; padding rows ignored               */
+  FstRows dq;            /* outputs                                          */
+  FstRows dk;
+  FstRows dv;
+  const float* lse;      /* from fst_grouped_forward                         */
+  float* delta;          /* output: D_i = dout_i . out_i                     */
+} FstGroupedBackwardArgs;
+
+int fst_grouped_forward(const FstGroupedForwardArgs* args, void* stream);
+int fst_grouped_backward(const FstGroupedBackwardArgs* args, void* stream);
+
+/* ---- rotary positions (no upstream counterpart) ----------------------------
+ *
+ * Rotates the first 2 * pairs channels of each row of q and k by the angle
+ * position * freqs[p], times magnitude: for the channels (a, b) of pair p,
+ *   a' = m (a cos t - b sin t),  b' = m (b cos t + a sin t),  t = pos * freqs[p]
+ * (a, b) = (x[p], x[p + pairs]), or (x[2p], x[2p + 1]) when interleaved. The
+ * remaining channels are copied. `inverse` rotates by -t: the gradient. The
+ * angle is reduced in fp64, so far positions keep their phase. Outputs may be
+ * the inputs themselves. k.data may be NULL (q alone).
+ */
+typedef struct FstRotaryArgs {
+  int32_t dtype;          /* enum FstDtype                                   */
+  int32_t packed;         /* 0 padded, 1 packed                              */
+  int32_t batch;          /* B (packed: events of cu_seqlens)                */
+  int32_t heads;          /* heads of q                                      */
+  int32_t kv_heads;       /* heads of k                                      */
+  int32_t max_len;        /* padded: L                                       */
+  int32_t head_dim;       /* Dh, 1 to 1024                                   */
+  int32_t pairs;          /* rotated channel pairs, 2 * pairs <= Dh          */
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t positions_64;   /* positions are int64 (else int32)                */
+  float magnitude;
+  int64_t total_rows;     /* padded: B*L. packed: T                          */
+  const double* freqs;       /* [pairs] device, radians per position          */
+  const int32_t* cu_seqlens; /* packed, [B+1] device: a row's position counts */
+                             /* from its event's start; rows of no event are  */
+                             /* copied. Ignored when positions is given       */
+  const void* positions;     /* [B, L] or [T] device, or NULL (padded: the row */
+                             /* index)                                        */
+  FstRows q;
+  FstRows k;
+  FstRows q_out;
+  FstRows k_out;
+} FstRotaryArgs;
+
+int fst_rotary(const FstRotaryArgs* args, void* stream);
 
 /* Number of CUDA kernels this library has launched in the process so far
  * (benchmark bookkeeping; no counterpart upstream). */

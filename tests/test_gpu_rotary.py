@@ -1,0 +1,151 @@
+"""Rotary positions against the float64 definition.
+
+A result is x cos - y sin in fp32 from cos and sin that are off by at most
+2^-22 (the reduced angle's rounding, 2^-25 turns = 1.9e-7 rad, and two ulp of
+sincospi, times the magnitude m), rounded once: the bound is
+u |ref| + 2^-21 m (|x| + |y|), u half a step of the type.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from flash_spacetime import (flash_rotary, flash_rotary_varlen, rotary_frequencies,
+                                 rotary_magnitude, rotary_reference)
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _check(got, x, freqs, pos, interleaved, mag):
+    x, got = x.detach().cpu(), got.detach().cpu()
+    pos = pos.cpu()
+    assert got.dtype == x.dtype and got.shape == x.shape
+    ref = rotary_reference(x.double(), freqs, pos, interleaved, mag)
+    rot = 2 * freqs.numel()
+    part = torch.zeros_like(ref)
+    head = x[..., :rot].double().abs()
+    if interleaved:
+        part[..., :rot] = head.unflatten(-1, (-1, 2)).sum(-1).repeat_interleave(2, -1)
+    else:
+        half = head.unflatten(-1, (2, -1)).sum(-2)
+        part[..., :rot] = torch.cat((half, half), -1)
+    bound = torch.finfo(x.dtype).eps / 2 * ref.abs() + 2.0**-21 * mag * part
+    bound += torch.finfo(x.dtype).tiny
+    worst = ((got.double() - ref).abs() / bound).max().item() if x.numel() else 0.0
+    assert worst <= 1.0, f"error {worst:.2f} times its bound"
+    assert torch.equal(got[..., rot:], x[..., rot:])
+
+
+def _event_positions(lens):
+    return torch.cat([torch.arange(n) for n in lens])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim, rot", [(32, 32), (32, 16), (64, 24), (128, 128), (48, 20), (80, 40),
+                                      (7, 6), (33, 2), (256, 256), (16, 0), (2, 2), (1024, 1024)])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_packed(dtype, dim, rot, interleaved):
+    lens = [5, 1, 0, 70, 33]
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    t = [torch.randn(sum(lens), h, dim, device="cuda", generator=gen).to(dtype)
+         for h in (3, 1, 3, 1)]
+    q, k = (x.requires_grad_(True) for x in t[:2])
+    freqs = rotary_frequencies(rot) if rot else torch.zeros(0, dtype=torch.float64)
+    cu = torch.tensor([0, 5, 6, 6, 76, 109], dtype=torch.int64, device="cuda")
+    outs = flash_rotary_varlen(q, k, freqs, cu, interleaved=interleaved, magnitude=1.25)
+    pos = _event_positions(lens)[:, None]
+    for got, x in zip(outs, (q, k)):
+        _check(got, x, freqs, pos, interleaved, 1.25)
+    for got, g in zip(torch.autograd.grad(outs, (q, k), t[2:]), t[2:]):
+        _check(got, g, -freqs, pos, interleaved, 1.25)
+
+
+@pytest.mark.parametrize("layout", ["bhld", "blhd"])
+@pytest.mark.parametrize("where", ["rows", "given", "shared"])
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (FP32, 48), (FP16, 10)])
+def test_padded(dtype, dim, where, layout):
+    b, n = 3, 37
+    shape = (lambda h: (b, h, n, dim) if layout == "bhld" else (b, n, h, dim))
+    q, k = (torch.randn(shape(h), device="cuda").to(dtype).requires_grad_(True) for h in (4, 2))
+    freqs = rotary_frequencies(dim, scaling="linear", factor=4.0)
+    pos = {"rows": None, "given": torch.randint(-50, 9999, (b, n)),
+           "shared": torch.randint(0, 99, (n,))}[where]
+    outs = flash_rotary(q, k, freqs, None if pos is None else pos.cuda(), layout=layout)
+    ref = torch.arange(n).expand(b, n) if pos is None else pos.expand(b, n)
+    ref = ref[:, None] if layout == "bhld" else ref[:, :, None]
+    for got, x in zip(outs, (q, k)):
+        _check(got, x, freqs, ref, False, 1.0)
+
+
+@pytest.mark.parametrize("start", [65519, 999983, 2**31 - 41, 2**40])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_far_positions_keep_their_phase(dtype, start):
+    # fp64 turns: off by 2^-52 of the angle, 2^-52 * 2^40 = 2^-12 turns at the
+    # farthest, which is only held to that.
+    x = torch.randn(40, 2, 64, device="cuda").to(dtype)
+    freqs = rotary_frequencies(64, scaling="parts", factor=32.0)
+    pos = start + torch.arange(40)
+    got, none = flash_rotary_varlen(x, None, freqs, positions=pos.cuda(),
+                                    magnitude=rotary_magnitude(32.0))
+    assert none is None
+    if start < 2**32:
+        _check(got, x, freqs, pos[:, None], False, rotary_magnitude(32.0))
+    else:
+        ref = rotary_reference(x.double().cpu(), freqs, pos[:, None], False,
+                               rotary_magnitude(32.0))
+        assert (got.double().cpu() - ref).abs().max() <= 2.0**-8 * ref.abs().max() + 2.0**-7
+
+
+def test_rows_of_no_event_are_copied():
+    x = torch.randn(20, 2, 32, device="cuda")
+    cu = torch.tensor([4, 9, 15], dtype=torch.int32, device="cuda")
+    got, _ = flash_rotary_varlen(x, None, rotary_frequencies(32), cu, magnitude=2.0)
+    assert torch.equal(got[:4], x[:4]) and torch.equal(got[15:], x[15:])
+    _check(got[9:15], x[9:15], rotary_frequencies(32), torch.arange(6)[:, None], False, 2.0)
+
+
+def test_strides_and_partial_gradients():
+    fused = torch.randn(50, 8, 32, device="cuda", dtype=BF16)
+    q, k, _ = fused.split((4, 2, 2), 1)
+    freqs, cu = rotary_frequencies(32), torch.tensor([0, 20, 50], device="cuda")
+    want = flash_rotary_varlen(q.contiguous(), k.contiguous(), freqs, cu)
+    got = flash_rotary_varlen(q, k, freqs, cu)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    odd = torch.zeros(50 * 4 * 32 + 1, device="cuda", dtype=BF16)[1:].view(50, 4, 32)
+    odd.copy_(q)
+    assert torch.equal(flash_rotary_varlen(odd, None, freqs, cu)[0], want[0])
+    apart = torch.zeros(50, 4, 32, 2, device="cuda", dtype=BF16)[..., 0]
+    apart.copy_(q)
+    assert torch.equal(flash_rotary_varlen(apart, None, freqs, cu)[0], want[0])
+    kl = k.contiguous().requires_grad_(True)
+    outs = flash_rotary_varlen(q, kl, freqs, cu)
+    (g,) = torch.autograd.grad(outs[1].float().sum(), kl)
+    _check(g, torch.ones_like(kl), -freqs, _event_positions([20, 30])[:, None], False, 1.0)
+
+
+def test_rotation_preserves_dot_products_of_equal_offsets():
+    # <R_i q, R_j k> depends on i - j alone: shifting both positions changes
+    # nothing but fp32 rounding (64 products of order 1 at 2^-21).
+    q, k = (torch.randn(1, 1, 1, 64, device="cuda").expand(1, 1, 9, 64) for _ in range(2))
+    freqs = rotary_frequencies(64)
+    near = flash_rotary(q, k, freqs, torch.arange(9, device="cuda"))
+    far = flash_rotary(q, k, freqs, torch.arange(9, device="cuda") + 123456)
+    dots = [(a.double() @ b.double().transpose(-1, -2)) for a, b in (near, far)]
+    scale = (q.abs().double() @ k.abs().double().transpose(-1, -2)).max()
+    assert (dots[0] - dots[1]).abs().max() <= 2.0**-18 * scale
+
+
+def test_graph_replay():
+    x = torch.randn(64, 2, 32, device="cuda", dtype=BF16)
+    freqs = rotary_frequencies(32).cuda()
+    cu = torch.tensor([0, 30, 64], dtype=torch.int32, device="cuda")
+    fixed = torch.zeros_like(x)
+    flash_rotary_varlen(fixed, None, freqs, cu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = flash_rotary_varlen(fixed, None, freqs, cu)
+    fixed.copy_(x)
+    graph.replay()
+    assert torch.equal(out, flash_rotary_varlen(x, None, freqs, cu)[0])
