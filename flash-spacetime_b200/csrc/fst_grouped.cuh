@@ -105,6 +105,10 @@ __device__ __forceinline__ int64_t stat_at(const FstGroupedProblem& p, const Row
 // Host side (fst_grouped_simt.cu, fst_grouped_fwd.cu, fst_grouped_bwd.cu).
 int simt_forward(const FstGroupedForwardArgs& a, cudaStream_t st);
 int simt_backward(const FstGroupedBackwardArgs& a, cudaStream_t st);
+// Whether the tensor-core kernels take a call: 16-bit, Dh a multiple of 8, and
+// every tensor on the 16-byte grid that TMA and the vector stores need.
+bool tc_takes(const FstGroupedForwardArgs& a);
+int tc_forward(const FstGroupedForwardArgs& a, cudaStream_t st);
 
 }  // namespace grouped
 }  // namespace fst

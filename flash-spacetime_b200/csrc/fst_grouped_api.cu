@@ -98,7 +98,8 @@ int fst_grouped_forward(const FstGroupedForwardArgs* a, void* stream) {
     return api_fail(FST_ERR_INVALID, "grouped forward: q, k, v, out and lse are required");
   cudaGetLastError();  // clear a stale error so the check below is ours
   const cudaStream_t st = (cudaStream_t)stream;
-  const int done = fst::grouped::simt_forward(*a, st);
+  const int done = fst::grouped::tc_takes(*a) ? fst::grouped::tc_forward(*a, st)
+                                              : fst::grouped::simt_forward(*a, st);
   return done ? done : status("grouped forward launch");
 }
 

@@ -1,0 +1,291 @@
+// Grouped-head attention, forward, on the tensor cores (16-bit inputs).
+//
+// One block owns 128 query rows of one event and head and walks the event's
+// keys in tiles of BN, twice resident on each SM so that one block's softmax
+// runs beside the other's products:
+//   warp 4   brings Q once and the K and V tiles by TMA;
+//   warp 5   issues S = Q K^T into tensor memory and O += P V from it;
+//   warps 0-3, one thread a query row: reads S, keeps the running maximum and
+//            sum, writes P back over S as 16-bit values (the A operand of the
+//            second product), rescales O when the maximum has grown.
+//
+// Softmax in the base-2 domain: p = 2^(c s - c m), c = |scale| log2(e) (the
+// sign of the scale is the product's own negate bit). O and l are rescaled
+// only when the maximum has grown by more than 2^8 since the last rescale:
+// p <= 2^8 then, exact in effect because the same m divides out at the end.
+//
+// P is rounded to the input type for the second product (u of its type, the
+// one rounding besides the output's); l sums the unrounded fp32 values.
+
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+#include "fst_grouped_tc.cuh"
+
+namespace fst {
+namespace grouped {
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kThreads = 192;
+constexpr float kGrow = 8.f;  // log2 of the growth that forces a rescale
+
+template <int Boxes, int BN, int Stages>
+struct FwdSmem {
+  alignas(1024) char q[Boxes * kBM * 128];
+  alignas(1024) char k[Stages][Boxes * BN * 128];
+  alignas(1024) char v[Stages][Boxes * BN * 128];
+  uint64_t q_full, k_full[Stages], k_empty[Stages], v_full[Stages], v_empty[Stages];
+  uint64_t s_full, p_ready, o_full;
+  uint32_t tmem;
+};
+
+template <typename T, int Boxes, int BN, int Stages>
+__global__ void __launch_bounds__(kThreads, 2)
+    fwd_kernel(const __grid_constant__ TileMaps maps, const FstGroupedForwardArgs a, int blocks) {
+  using Smem = FwdSmem<Boxes, BN, Stages>;
+  extern __shared__ char raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  constexpr int kCols = 256;  // S (P over it) in [0, BN), O in [128, 128 + Dh)
+  const FstGroupedProblem& p = a.prob;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const BlockAt at = block_at(p, blocks);
+  RowTile t;
+  if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
+  const int D = p.head_dim;
+  if (t.i0 + kBM > t.len) {
+    // Rows of no event in this block: zeros.
+    const int first = max(t.i0, t.len), n = min(t.i0 + kBM, t.lim) - first;
+    for (int e = threadIdx.x; e < n * (D / 8); e += kThreads)
+      *(uint4*)(row_ptr<T>(a.out, t, at.h, first + e / (D / 8)) + e % (D / 8) * 8) =
+          make_uint4(0, 0, 0, 0);
+    if (t.i0 >= t.len) return;
+  }
+  const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
+  const int tiles = (end + BN - 1) / BN;
+
+  if (warp == 4) {
+    tmem_alloc<kCols>(smem_addr(&sm.tmem));
+  } else if (threadIdx.x == 0) {
+    mbar_init(smem_addr(&sm.q_full), 1);
+    for (int s = 0; s < Stages; ++s) {
+      mbar_init(smem_addr(&sm.k_full[s]), 1);
+      mbar_init(smem_addr(&sm.k_empty[s]), 1);
+      mbar_init(smem_addr(&sm.v_full[s]), 1);
+      mbar_init(smem_addr(&sm.v_empty[s]), 1);
+    }
+    mbar_init(smem_addr(&sm.s_full), 1);
+    mbar_init(smem_addr(&sm.p_ready), 4);
+    mbar_init(smem_addr(&sm.o_full), 1);
+    mbar_init_fence();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const uint32_t tS = tmem, tO = tmem + 128;
+
+  bool ok = true;
+  if (warp == 4) {
+    if (lane == 0) {
+      load_tile<Boxes, kBM>(smem_addr(sm.q), &maps.q, smem_addr(&sm.q_full), t.base + t.i0, at.h,
+                            t.ev);
+      for (int it = 0; it < tiles && ok; ++it) {
+        const int s = it % Stages, round = it / Stages;
+        if (round) ok = mbar_wait(smem_addr(&sm.k_empty[s]), (round - 1) & 1);
+        if (!ok) break;
+        load_tile<Boxes, BN>(smem_addr(sm.k[s]), &maps.k, smem_addr(&sm.k_full[s]),
+                             t.base + it * BN, at.kh, t.ev);
+        if (round) ok = mbar_wait(smem_addr(&sm.v_empty[s]), (round - 1) & 1);
+        if (!ok) break;
+        load_tile<Boxes, BN>(smem_addr(sm.v[s]), &maps.v, smem_addr(&sm.v_full[s]),
+                             t.base + it * BN, at.kh, t.ev);
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      const uint32_t o_instr = instruction<T>((D + 15) & ~15, true, false);
+      ok = mbar_wait(smem_addr(&sm.q_full), 0);
+      for (int it = 0; it < tiles && ok; ++it) {
+        const int s = it % Stages, parity = (it / Stages) & 1;
+        const int steps = (min(BN, end - it * BN) + 15) / 16;  // of 16 keys
+        ok = mbar_wait(smem_addr(&sm.k_full[s]), parity);
+        if (!ok) break;
+        // S may be overwritten: MMAs complete in order, so the product that
+        // read P from it is done before this one writes.
+        const uint32_t s_instr = instruction<T>(steps * 16, false, p.scale < 0.f);
+        for (int c = 0; c * 16 < D; ++c)
+          mma_ss(tS, operand(smem_addr(sm.q) + (c / 4) * kBM * 128 + (c % 4) * 32, 0),
+                 operand(smem_addr(sm.k[s]) + (c / 4) * BN * 128 + (c % 4) * 32, 0), s_instr,
+                 c > 0);
+        tc_commit(smem_addr(&sm.s_full));
+        tc_commit(smem_addr(&sm.k_empty[s]));
+        ok = mbar_wait(smem_addr(&sm.v_full[s]), parity) &&
+             mbar_wait(smem_addr(&sm.p_ready), it & 1);
+        if (!ok) break;
+        tc_fence_after();
+        for (int c = 0; c < steps; ++c)
+          mma_ts(tO, tS + c * 8, operand(smem_addr(sm.v[s]) + c * 2048, BN * 128), o_instr,
+                 it > 0 || c > 0);
+        tc_commit(smem_addr(&sm.v_empty[s]));
+      }
+      if (ok) tc_commit(smem_addr(&sm.o_full));
+    }
+  } else {
+    const uint32_t quad = (uint32_t)(warp * 32) << 16;
+    const int i = t.i0 + warp * 32 + lane;
+    // Above 0, so that a masked -inf stays -inf under a scale of 0.
+    const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
+    float m = -INFINITY, l = 0.f;
+    for (int it = 0; it < tiles; ++it) {
+      const int j0 = it * BN, nk = min(BN, end - j0);
+      // Keys j0 <= j < j0 + lim are seen; `edge` when some row sees fewer
+      // than the tile's keys.
+      const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
+      const bool edge = j0 + BN > t.len || (p.causal && j0 + BN > t.i0 + 1);
+      ok = mbar_wait(smem_addr(&sm.s_full), it & 1);
+      if (!ok) break;
+      tc_fence_after();
+      float s[BN / 32][32];
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c)
+        if (c * 32 < nk) tmem_ld32(s[c], tS + quad + c * 32);
+      tmem_wait_ld();
+      float mx = m;
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        if (c * 32 >= nk) continue;
+        pin(s[c]);
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e < lim ? s[c][e] : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[c][e]);
+      }
+      // First tile: O is written, not added to, so m may move freely.
+      if (it == 0) {
+        m = mx;
+      } else {
+        const bool grow = (mx - m) * c2 > kGrow || (m == -INFINITY && mx > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float keep = grow ? ex2((m - mx) * c2) : 1.f;
+          if (grow) {
+            m = mx;
+            l *= keep;
+          }
+#pragma unroll 1
+          for (int d = 0; d < D; d += 16) tmem_scale16(tO + quad + d, keep);
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : m * c2;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        if (c * 32 >= nk) continue;
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float x = ex2(fmaf(s[c][e], c2, -off)), y = ex2(fmaf(s[c][e + 1], c2, -off));
+          sum += x + y;
+          w[e / 2] = Elem<T>::pack(x, y);
+        }
+        tmem_st16(tS + quad + c * 16, w);
+      }
+      l += sum;
+      if (nk & 15) {
+        // Keys up to the next multiple of 16 have p = 0, but what V holds
+        // there (another event's rows) must not be able to make 0 * NaN.
+        const int st = it % Stages;
+        ok = mbar_wait(smem_addr(&sm.v_full[st]), (it / Stages) & 1);
+        if (!ok) break;
+        zero_tile_rows<Boxes, BN>(sm.v[st], nk, (nk + 15) & ~15, threadIdx.x, 128);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&sm.p_ready));
+    }
+    if (ok) ok = mbar_wait(smem_addr(&sm.o_full), 0);
+    tc_fence_after();
+    const bool live = i < t.len;
+    T* out = live ? row_ptr<T>(a.out, t, at.h, i) : nullptr;
+    const float inv = ok ? 1.f / l : NAN;
+    for (int d = 0; d < D; d += 32) {
+      float o[32];
+      tmem_ld32(o, tO + quad + d);
+      tmem_wait_ld();
+      pin(o);
+      if (!live) continue;
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        if (d + e >= D) break;
+        uint4 w;
+        w.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
+        w.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+        w.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+        w.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+        *(uint4*)(out + d + e) = w;
+      }
+    }
+    if (live) a.lse[stat_at(p, t, p.heads, at.h, i)] = ok ? (m * c2 + log2f(l)) / kLog2e : NAN;
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 4) tmem_free<kCols>(tmem);
+}
+
+template <typename T, int Boxes, int BN, int Stages>
+int launch(const FstGroupedForwardArgs& a, cudaStream_t st) {
+  const FstGroupedProblem& p = a.prob;
+  static std::atomic<uint64_t> done{0};
+  const auto kernel = fwd_kernel<T, Boxes, BN, Stages>;
+  const int bytes = (int)sizeof(FwdSmem<Boxes, BN, Stages>) + 1024;
+  const int e = allow_dynamic_smem((const void*)kernel, bytes, done);
+  if (e) return api_fail(FST_ERR_CUDA, "shared memory: %s", cudaGetErrorString((cudaError_t)e));
+  const int64_t rows = p.packed ? p.total_rows : p.max_len, events = p.packed ? 1 : p.batch;
+  TileMaps maps;
+  int rc = tc::make_rows_map(&maps.q, a.q, p.head_dim, rows, p.heads, events, kBM);
+  if (!rc) rc = tc::make_rows_map(&maps.k, a.k, p.head_dim, rows, p.kv_heads, events, BN);
+  if (!rc) rc = tc::make_rows_map(&maps.v, a.v, p.head_dim, rows, p.kv_heads, events, BN);
+  if (rc) return rc;
+  maps.g = maps.q;
+  const int blocks = (int)list_blocks(p, kBM);
+  kernel<<<(unsigned)(blocks * p.heads), kThreads, bytes, st>>>(maps, a, blocks);
+  count_launch();
+  return FST_OK;
+}
+
+template <typename T>
+int launch_t(const FstGroupedForwardArgs& a, cudaStream_t st) {
+  if (a.prob.head_dim <= 64) return launch<T, 1, 128, 2>(a, st);
+  return launch<T, 2, 128, 1>(a, st);
+}
+
+bool on_grid(const FstRows& r, int64_t rows, int heads, int64_t events) {
+  auto good = [](int64_t n, int64_t stride) {
+    return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38));
+  };
+  return ((uintptr_t)r.data & 15) == 0 && good(rows, r.row_stride) && good(heads, r.head_stride) &&
+         good(events, r.event_stride);
+}
+
+}  // namespace
+
+bool tc_takes(const FstGroupedForwardArgs& a) {
+  const FstGroupedProblem& p = a.prob;
+  if (p.dtype == FST_F32 || p.head_dim % 8) return false;
+  const int64_t rows = p.packed ? p.total_rows : p.max_len, events = p.packed ? 1 : p.batch;
+  return on_grid(a.q, rows, p.heads, events) && on_grid(a.out, rows, p.heads, events) &&
+         on_grid(a.k, rows, p.kv_heads, events) && on_grid(a.v, rows, p.kv_heads, events);
+}
+
+int tc_forward(const FstGroupedForwardArgs& a, cudaStream_t st) {
+  if (a.prob.dtype == FST_BF16) return launch_t<__nv_bfloat16>(a, st);
+  return launch_t<__half>(a, st);
+}
+
+}  // namespace grouped
+}  // namespace fst

@@ -1,0 +1,209 @@
+// Grouped-head attention on the 5th-generation tensor cores: the pieces that
+// its forward and backward kernels share (tcgen05, TMEM, TMA, work order).
+//
+// A tile is rows of one head's [rows, Dh] slice, brought by TMA in boxes of 64
+// channels (128 bytes a row, 128-byte swizzle); channels past Dh and rows past
+// the tensor read as zeros, so every Dh that is a multiple of 8 up to 128
+// runs on the same code, with one box (Dh <= 64) or two. Products use
+// kind::f16 with fp32 accumulators in tensor memory.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "fst_grouped.cuh"
+#include "fst_tc_common.cuh"
+
+namespace fst {
+namespace grouped {
+
+using tc::Elem;
+using tc::ex2;
+using tc::fence_proxy_async;
+using tc::mbar_arrive_tx;
+using tc::mbar_init;
+using tc::mbar_init_fence;
+using tc::mbar_wait;
+
+// Tensor maps of a launch (make_rows_map), passed as a kernel parameter.
+struct __align__(64) TileMaps {
+  CUtensorMap q, k, v, g;
+};
+
+// ---- tcgen05 ----------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Whole warp. The address of the allocation is written to `slot`.
+template <int Cols>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+               "n"(Cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int Cols>
+__device__ __forceinline__ void tmem_free(uint32_t addr) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "n"(Cols));
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// Arrives on `bar` when every MMA this thread has issued so far is complete.
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+
+// Shared-memory operand in the 128-byte swizzle: start address, leading and
+// stride byte offsets in units of 16 bytes, descriptor version 1.
+// K-major (rows of 64 channels, the product runs along the channels): 8-row
+// groups are 1024 bytes apart. MN-major (the product runs along the rows): the
+// same 8-row groups are the stride, and `lead` separates boxes of 64 channels.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 |
+         (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor: fp32 accumulator, A and B of type T, M = 128.
+template <typename T>
+__device__ __forceinline__ uint32_t instruction(int n, bool b_mn_major, bool negate) {
+  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  return 1u << 4 | type << 7 | type << 10 | (negate ? 1u << 13 : 0) |
+         (b_mn_major ? 1u << 16 : 0) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((int)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((int)add)
+      : "memory");
+}
+
+// 32 columns of the warp's 32 lanes (one row a thread). The values may be
+// read after tmem_wait_ld().
+__device__ __forceinline__ void tmem_ld32(float (&r)[32], uint32_t addr) {
+  uint32_t* x = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]),
+        "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]),
+        "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]),
+        "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]),
+        "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&x)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]),
+      "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]),
+      "r"(x[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// 16 columns in place: each row times its factor. Waits for itself.
+__device__ __forceinline__ void tmem_scale16(uint32_t addr, float f) {
+  uint32_t x[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]),
+        "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]),
+        "=r"(x[14]), "=r"(x[15])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+  tmem_st16(addr, x);
+}
+// Keeps the uses of loaded registers behind the tmem_wait_ld() before it.
+__device__ __forceinline__ void pin(float (&x)[32]) {
+  asm volatile(""
+               : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]),
+                 "+f"(x[6]), "+f"(x[7]), "+f"(x[8]), "+f"(x[9]), "+f"(x[10]), "+f"(x[11]),
+                 "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15]));
+  asm volatile(""
+               : "+f"(x[16]), "+f"(x[17]), "+f"(x[18]), "+f"(x[19]), "+f"(x[20]), "+f"(x[21]),
+                 "+f"(x[22]), "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]),
+                 "+f"(x[28]), "+f"(x[29]), "+f"(x[30]), "+f"(x[31]));
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// ---- TMA --------------------------------------------------------------------
+
+// Box of 64 channels from `c` (a multiple of 64: 128 bytes), rows from `row`
+// of head `h` of event `ev`. Rows and channels past the tensor read as zeros.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c,
+                                         int row, int h, int ev) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c), "r"(row), "r"(h), "r"(ev)
+      : "memory");
+}
+// All boxes of a tile of `Rows` rows.
+template <int Boxes, int Rows>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                          int row, int h, int ev) {
+  mbar_arrive_tx(bar, Boxes * Rows * 128);
+#pragma unroll
+  for (int b = 0; b < Boxes; ++b) load_box(dst + b * Rows * 128, map, bar, b * 64, row, h, ev);
+}
+
+// Zeros rows [first, last) of a tile (whole rows, so the swizzle does not
+// matter), by `n` threads of index t; made visible to the tensor cores.
+template <int Boxes, int Rows>
+__device__ __forceinline__ void zero_tile_rows(char* tile, int first, int last, int t, int n) {
+  for (int e = t; e < (last - first) * 8 * Boxes; e += n) {
+    const int b = e / ((last - first) * 8), r = e - b * (last - first) * 8;
+    *(uint4*)(tile + b * Rows * 128 + first * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
+}
+
+// Head and work-list position of a block: key heads outermost (their K and V
+// stay in L2), the query heads of a group innermost (they share them).
+struct BlockAt {
+  int kh, h, id;
+};
+__device__ __forceinline__ BlockAt block_at(const FstGroupedProblem& p, int blocks) {
+  const int group = p.heads / p.kv_heads;
+  BlockAt b;
+  const int x = blockIdx.x / group;
+  b.kh = x / blocks;
+  b.id = x - b.kh * blocks;
+  b.h = b.kh * group + (blockIdx.x - x * group);
+  return b;
+}
+
+}  // namespace grouped
+}  // namespace fst

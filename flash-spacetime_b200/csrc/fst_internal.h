@@ -35,6 +35,11 @@ namespace tc {
 // for the row-interleaved layouts. Only Dh in {16, 32, 64} (tma_shape).
 bool tma_shape(int dh);
 int make_head_map(CUtensorMap* map, const FstProblem& p, const void* base, int row_elems);
+// TMA tensor map of a 16-bit [events, heads, rows, Dh] tensor, any strides:
+// boxes of 64 channels x box_rows rows in the 128-byte swizzle. Channels past
+// Dh and rows past the tensor read as zeros.
+int make_rows_map(CUtensorMap* map, const FstRows& t, int dh, int64_t rows, int heads,
+                  int64_t events, int box_rows);
 bool fwd_supported(const FstProblem& p);
 size_t fwd_workspace(const FstProblem& p);
 int launch_fwd(const FstForwardArgs& a, cudaStream_t st);

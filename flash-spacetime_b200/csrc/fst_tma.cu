@@ -40,6 +40,43 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 }  // namespace
 
+// Runs an encode call, giving the thread a driver context first if it has none:
+// a thread that has made no runtime call yet (PyTorch runs backward on its own
+// device threads) has no current driver context, so the current device's
+// primary context is bound, as the runtime would, and the call retried.
+template <typename F>
+static CUresult with_context(F run) {
+  CUresult r = run();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = run();
+  }
+  return r;
+}
+
+int make_rows_map(CUtensorMap* map, const FstRows& t, int dh, int64_t rows, int heads,
+                  int64_t events, int box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 encode = encode_fn();
+  if (!encode) return api_fail(FST_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[4] = {(cuuint64_t)dh, (cuuint64_t)rows, (cuuint64_t)heads,
+                              (cuuint64_t)events};
+  // The stride of an axis of one entry is never used, but has to be valid.
+  auto bytes = [](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 ? stride * 2 : 256); };
+  const cuuint64_t strides[3] = {bytes(rows, t.row_stride), bytes(heads, t.head_stride),
+                                 bytes(events, t.event_stride)};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)box_rows, 1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = with_context([&] {
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, t.data, dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+  if (r != CUDA_SUCCESS)
+    return api_fail(FST_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for [%lld, %d, %lld, %d]",
+                    (int)r, (long long)events, heads, (long long)rows, dh);
+  return FST_OK;
+}
+
 bool tma_shape(int dh) { return dh == 16 || dh == 32 || dh == 64; }
 
 int make_head_map(CUtensorMap* map, const FstProblem& p, const void* base, int row_elems) {
@@ -68,14 +105,7 @@ int make_head_map(CUtensorMap* map, const FstProblem& p, const void* base, int r
                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
-  CUresult r = run();
-  if (r == CUDA_ERROR_INVALID_CONTEXT) {
-    // A thread that has made no runtime call yet (PyTorch runs backward on
-    // its own device threads) has no current driver context: bind the
-    // current device's primary context, as the runtime would, and retry.
-    int dev = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = run();
-  }
+  const CUresult r = with_context(run);
   if (r != CUDA_SUCCESS)
     return api_fail(FST_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for a [%llu x %llu] view",
                     (int)r, (unsigned long long)dims[1], (unsigned long long)dims[0]);
