@@ -108,7 +108,9 @@ int simt_backward(const FstGroupedBackwardArgs& a, cudaStream_t st);
 // Whether the tensor-core kernels take a call: 16-bit, Dh a multiple of 8, and
 // every tensor on the 16-byte grid that TMA and the vector stores need.
 bool tc_takes(const FstGroupedForwardArgs& a);
+bool tc_takes(const FstGroupedBackwardArgs& a);
 int tc_forward(const FstGroupedForwardArgs& a, cudaStream_t st);
+int tc_backward(const FstGroupedBackwardArgs& a, cudaStream_t st);
 
 }  // namespace grouped
 }  // namespace fst

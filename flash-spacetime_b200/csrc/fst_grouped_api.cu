@@ -113,7 +113,8 @@ int fst_grouped_backward(const FstGroupedBackwardArgs* a, void* stream) {
     return api_fail(FST_ERR_INVALID, "grouped backward: a required pointer is null");
   cudaGetLastError();
   const cudaStream_t st = (cudaStream_t)stream;
-  const int done = fst::grouped::simt_backward(*a, st);
+  const int done = fst::grouped::tc_takes(*a) ? fst::grouped::tc_backward(*a, st)
+                                              : fst::grouped::simt_backward(*a, st);
   return done ? done : status("grouped backward launch");
 }
 

@@ -54,14 +54,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   RowTile t;
   if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
   const int D = p.head_dim;
-  if (t.i0 + kBM > t.len) {
-    // Rows of no event in this block: zeros.
-    const int first = max(t.i0, t.len), n = min(t.i0 + kBM, t.lim) - first;
-    for (int e = threadIdx.x; e < n * (D / 8); e += kThreads)
-      *(uint4*)(row_ptr<T>(a.out, t, at.h, first + e / (D / 8)) + e % (D / 8) * 8) =
-          make_uint4(0, 0, 0, 0);
-    if (t.i0 >= t.len) return;
-  }
+  zero_dead_rows<T, kBM>(a.out, t, at.h, D, kThreads);
+  if (t.i0 >= t.len) return;
   const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
   const int tiles = (end + BN - 1) / BN;
 
@@ -89,18 +83,20 @@ __global__ void __launch_bounds__(kThreads, 2)
   bool ok = true;
   if (warp == 4) {
     if (lane == 0) {
-      load_tile<Boxes, kBM>(smem_addr(sm.q), &maps.q, smem_addr(&sm.q_full), t.base + t.i0, at.h,
-                            t.ev);
+      const uint32_t q_full = smem_addr(&sm.q_full);
+      mbar_arrive_tx(q_full, Boxes * kBM * 128);
+      load_boxes<Boxes, kBM>(smem_addr(sm.q), &maps.q, q_full, t.base + t.i0, at.h, t.ev);
       for (int it = 0; it < tiles && ok; ++it) {
         const int s = it % Stages, round = it / Stages;
+        const uint32_t k_full = smem_addr(&sm.k_full[s]), v_full = smem_addr(&sm.v_full[s]);
         if (round) ok = mbar_wait(smem_addr(&sm.k_empty[s]), (round - 1) & 1);
         if (!ok) break;
-        load_tile<Boxes, BN>(smem_addr(sm.k[s]), &maps.k, smem_addr(&sm.k_full[s]),
-                             t.base + it * BN, at.kh, t.ev);
+        mbar_arrive_tx(k_full, Boxes * BN * 128);
+        load_boxes<Boxes, BN>(smem_addr(sm.k[s]), &maps.k, k_full, t.base + it * BN, at.kh, t.ev);
         if (round) ok = mbar_wait(smem_addr(&sm.v_empty[s]), (round - 1) & 1);
         if (!ok) break;
-        load_tile<Boxes, BN>(smem_addr(sm.v[s]), &maps.v, smem_addr(&sm.v_full[s]),
-                             t.base + it * BN, at.kh, t.ev);
+        mbar_arrive_tx(v_full, Boxes * BN * 128);
+        load_boxes<Boxes, BN>(smem_addr(sm.v[s]), &maps.v, v_full, t.base + it * BN, at.kh, t.ev);
       }
     }
   } else if (warp == 5) {
@@ -114,11 +110,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!ok) break;
         // S may be overwritten: MMAs complete in order, so the product that
         // read P from it is done before this one writes.
-        const uint32_t s_instr = instruction<T>(steps * 16, false, p.scale < 0.f);
-        for (int c = 0; c * 16 < D; ++c)
-          mma_ss(tS, operand(smem_addr(sm.q) + (c / 4) * kBM * 128 + (c % 4) * 32, 0),
-                 operand(smem_addr(sm.k[s]) + (c / 4) * BN * 128 + (c % 4) * 32, 0), s_instr,
-                 c > 0);
+        product<T, Boxes, kBM, BN>(tS, smem_addr(sm.q), smem_addr(sm.k[s]), D, steps * 16,
+                                   p.scale < 0.f);
         tc_commit(smem_addr(&sm.s_full));
         tc_commit(smem_addr(&sm.k_empty[s]));
         ok = mbar_wait(smem_addr(&sm.v_full[s]), parity) &&
@@ -210,25 +203,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (ok) ok = mbar_wait(smem_addr(&sm.o_full), 0);
     tc_fence_after();
     const bool live = i < t.len;
-    T* out = live ? row_ptr<T>(a.out, t, at.h, i) : nullptr;
-    const float inv = ok ? 1.f / l : NAN;
-    for (int d = 0; d < D; d += 32) {
-      float o[32];
-      tmem_ld32(o, tO + quad + d);
-      tmem_wait_ld();
-      pin(o);
-      if (!live) continue;
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        if (d + e >= D) break;
-        uint4 w;
-        w.x = Elem<T>::pack(o[e] * inv, o[e + 1] * inv);
-        w.y = Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
-        w.z = Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
-        w.w = Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
-        *(uint4*)(out + d + e) = w;
-      }
-    }
+    store_row<T>(live ? row_ptr<T>(a.out, t, at.h, i) : nullptr, tO + quad, D,
+                 ok ? 1.f / l : NAN);
     if (live) a.lse[stat_at(p, t, p.heads, at.h, i)] = ok ? (m * c2 + log2f(l)) / kLog2e : NAN;
     tc_fence_before();
   }
@@ -264,22 +240,12 @@ int launch_t(const FstGroupedForwardArgs& a, cudaStream_t st) {
   return launch<T, 2, 128, 1>(a, st);
 }
 
-bool on_grid(const FstRows& r, int64_t rows, int heads, int64_t events) {
-  auto good = [](int64_t n, int64_t stride) {
-    return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38));
-  };
-  return ((uintptr_t)r.data & 15) == 0 && good(rows, r.row_stride) && good(heads, r.head_stride) &&
-         good(events, r.event_stride);
-}
-
 }  // namespace
 
 bool tc_takes(const FstGroupedForwardArgs& a) {
   const FstGroupedProblem& p = a.prob;
-  if (p.dtype == FST_F32 || p.head_dim % 8) return false;
-  const int64_t rows = p.packed ? p.total_rows : p.max_len, events = p.packed ? 1 : p.batch;
-  return on_grid(a.q, rows, p.heads, events) && on_grid(a.out, rows, p.heads, events) &&
-         on_grid(a.k, rows, p.kv_heads, events) && on_grid(a.v, rows, p.kv_heads, events);
+  return tc_type(p) && on_grid(p, a.q, p.heads) && on_grid(p, a.out, p.heads) &&
+         on_grid(p, a.k, p.kv_heads) && on_grid(p, a.v, p.kv_heads);
 }
 
 int tc_forward(const FstGroupedForwardArgs& a, cudaStream_t st) {

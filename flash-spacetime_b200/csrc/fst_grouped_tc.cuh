@@ -170,11 +170,10 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c), "r"(row), "r"(h), "r"(ev)
       : "memory");
 }
-// All boxes of a tile of `Rows` rows.
+// All boxes of a tile of `Rows` rows; Boxes * Rows * 128 bytes land on `bar`.
 template <int Boxes, int Rows>
-__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                          int row, int h, int ev) {
-  mbar_arrive_tx(bar, Boxes * Rows * 128);
+__device__ __forceinline__ void load_boxes(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                           int row, int h, int ev) {
 #pragma unroll
   for (int b = 0; b < Boxes; ++b) load_box(dst + b * Rows * 128, map, bar, b * 64, row, h, ev);
 }
@@ -189,6 +188,64 @@ __device__ __forceinline__ void zero_tile_rows(char* tile, int first, int last, 
   }
   fence_proxy_async();
 }
+
+// d[128][n] = A B^T over the D channels, both tiles K-major in shared memory.
+template <typename T, int Boxes, int ARows, int BRows>
+__device__ __forceinline__ void product(uint32_t d, uint32_t A, uint32_t B, int D, int n,
+                                        bool negate) {
+  const uint32_t instr = instruction<T>(n, false, negate);
+#pragma unroll
+  for (int c = 0; c < Boxes * 4; ++c)
+    if (c * 16 < D)
+      mma_ss(d, operand(A + (c / 4) * ARows * 128 + (c % 4) * 32, 0),
+             operand(B + (c / 4) * BRows * 128 + (c % 4) * 32, 0), instr, c > 0);
+}
+
+// The block's rows of no event: zeros, in 16-byte vectors, by n threads.
+template <typename T, int BM>
+__device__ __forceinline__ void zero_dead_rows(const FstRows& out, const RowTile& t, int h, int D,
+                                               int n) {
+  if (t.i0 + BM <= t.len) return;
+  const int first = max(t.i0, t.len), rows = min(t.i0 + BM, t.lim) - first;
+  for (int e = threadIdx.x; e < rows * (D / 8); e += n)
+    *(uint4*)(row_ptr<T>(out, t, h, first + e / (D / 8)) + e % (D / 8) * 8) =
+        make_uint4(0, 0, 0, 0);
+}
+
+// A thread's row of D accumulator columns, times f, rounded and stored (whole
+// warps; out may be null).
+template <typename T>
+__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f) {
+  for (int d = 0; d < D; d += 32) {
+    float o[32];
+    tmem_ld32(o, acc + d);
+    tmem_wait_ld();
+    pin(o);
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+      if (!out || d + e >= D) break;
+      uint4 w;
+      w.x = Elem<T>::pack(o[e] * f, o[e + 1] * f);
+      w.y = Elem<T>::pack(o[e + 2] * f, o[e + 3] * f);
+      w.z = Elem<T>::pack(o[e + 4] * f, o[e + 5] * f);
+      w.w = Elem<T>::pack(o[e + 6] * f, o[e + 7] * f);
+      *(uint4*)(out + d + e) = w;
+    }
+    __syncwarp();  // tcgen05.ld takes the whole warp
+  }
+}
+
+// Whether a tensor lies on the 16-byte grid that TMA and the vector stores
+// need (strides of axes of one entry are never used).
+inline bool on_grid(const FstGroupedProblem& p, const FstRows& r, int heads) {
+  auto good = [](int64_t n, int64_t stride) {
+    return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38));
+  };
+  return ((uintptr_t)r.data & 15) == 0 &&
+         good(p.packed ? p.total_rows : p.max_len, r.row_stride) && good(heads, r.head_stride) &&
+         good(p.packed ? 1 : p.batch, r.event_stride);
+}
+inline bool tc_type(const FstGroupedProblem& p) { return p.dtype != FST_F32 && p.head_dim % 8 == 0; }
 
 // Head and work-list position of a block: key heads outermost (their K and V
 // stay in L2), the query heads of a group innermost (they share them).
