@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       lse2 = a.lse[st] * kLog2e;
       a.delta[st] = delta;
     }
+    const pair_t scale2 = pair(c2, c2), lse2n = pair(-lse2, -lse2), delta2n = pair(-delta, -delta);
     for (int it = 0; it < tiles; ++it) {
       const int j0 = it * kBN, nk = min(kBN, end - j0);
       const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
@@ -158,9 +159,15 @@ __global__ void __launch_bounds__(kRowThreads, 2)
         pin(dp);
         uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float ds = ex2(fmaf(s[e], c2, -lse2)) * (dp[e] - delta);
-          s[e] = edge && c * 32 + e >= lim ? 0.f : ds;
+        for (int e = 0; e < 32; e += 2) {
+          float2 x = split(fma2(pair(s[e], s[e + 1]), scale2, lse2n));
+          x = split(mul2(pair(ex2(x.x), ex2(x.y)), add2(pair(dp[e], dp[e + 1]), delta2n)));
+          s[e] = x.x;
+          s[e + 1] = x.y;
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = c * 32 + e < lim ? s[e] : 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = Elem<T>::pack(s[2 * e], s[2 * e + 1]);
@@ -194,8 +201,8 @@ struct ColSmem {
   alignas(1024) char v[Boxes * kBM * 128];
   alignas(1024) char q[Stages][Boxes * kBN * 128];
   alignas(1024) char g[Stages][Boxes * kBN * 128];
-  alignas(16) float lse2[Stages][kBN];
-  alignas(16) float delta[Stages][kBN];
+  alignas(16) float lse2n[Stages][kBN];   // -log2(e) lse of the query rows
+  alignas(16) float deltan[Stages][kBN];  // -D
   uint64_t own_full, full[Stages], empty[Stages], s_full[Groups], ready[Groups], done;
   uint32_t tmem;
 };
@@ -270,8 +277,8 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
 #pragma unroll
       for (int r = lane; r < kBN; r += 32) {
         const bool live = q0 + r < t.len;
-        sm.lse2[s][r] = live ? a.lse[st + r] * kLog2e : 0.f;
-        sm.delta[s][r] = live ? a.delta[st + r] : 0.f;
+        sm.lse2n[s][r] = live ? a.lse[st + r] * -kLog2e : 0.f;
+        sm.deltan[s][r] = live ? -a.delta[st + r] : 0.f;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
@@ -321,6 +328,7 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
     const uint32_t tS = tmem + w * 128 + quad, tP = tS + 64;
     const int j = t.i0 + warp % 4 * 32 + lane;
     const float c2 = fabsf(p.scale) * kLog2e;
+    const pair_t scale2 = pair(c2, c2);
     for (int it = w; it < tiles; it += Groups) {
       const int s = it % Stages;
       const int q0 = first + it % per_head * kBN, nq = min(kBN, t.len - q0);
@@ -341,17 +349,27 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
         pin(dp);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          const float4 l4 = *(const float4*)&sm.lse2[s][c * 32 + e];
-          const float4 d4 = *(const float4*)&sm.delta[s][c * 32 + e];
-          const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w};
+          const ulonglong2 ls = *(const ulonglong2*)&sm.lse2n[s][c * 32 + e];
+          const ulonglong2 de = *(const ulonglong2*)&sm.deltan[s][c * 32 + e];
 #pragma unroll
-          for (int f = 0; f < 4; ++f) {
-            const int col = c * 32 + e + f;
-            const bool out = edge && (col < lo || col >= nq);
-            const float pr = ex2(fmaf(x[e + f], c2, -ls[f]));
-            const float ds = pr * (dp[e + f] - de[f]);
-            x[e + f] = out ? 0.f : pr;
-            dp[e + f] = out ? 0.f : ds;
+          for (int f = 0; f < 4; f += 2) {
+            float2 y = split(fma2(pair(x[e + f], x[e + f + 1]), scale2, f ? ls.y : ls.x));
+            y.x = ex2(y.x);
+            y.y = ex2(y.y);
+            const float2 ds = split(mul2(
+                pair(y.x, y.y), add2(pair(dp[e + f], dp[e + f + 1]), f ? de.y : de.x)));
+            x[e + f] = y.x;
+            x[e + f + 1] = y.y;
+            dp[e + f] = ds.x;
+            dp[e + f + 1] = ds.y;
+          }
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const bool seen = c * 32 + e >= lo && c * 32 + e < nq;
+            x[e] = seen ? x[e] : 0.f;
+            dp[e] = seen ? dp[e] : 0.f;
           }
         }
         uint32_t wp[16], wd[16];

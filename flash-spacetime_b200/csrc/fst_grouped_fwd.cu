@@ -4,7 +4,8 @@
 // keys in tiles of BN, twice resident on each SM so that one block's softmax
 // runs beside the other's products:
 //   warp 4   brings Q once and the K and V tiles by TMA;
-//   warp 5   issues S = Q K^T into tensor memory and O += P V from it;
+//   warp 5   issues S = Q K^T into tensor memory, one tile ahead (two S
+//            buffers), and O += P V from it;
 //   warps 0-3, one thread a query row: reads S, keeps the running maximum and
 //            sum, writes P back over S as 16-bit values (the A operand of the
 //            second product), rescales O when the maximum has grown.
@@ -37,7 +38,7 @@ struct FwdSmem {
   alignas(1024) char k[Stages][Boxes * BN * 128];
   alignas(1024) char v[Stages][Boxes * BN * 128];
   uint64_t q_full, k_full[Stages], k_empty[Stages], v_full[Stages], v_empty[Stages];
-  uint64_t s_full, p_ready, o_full;
+  uint64_t s_full[2], p_ready[2], pv_done[2];  // of even and odd tiles
   uint32_t tmem;
 };
 
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   using Smem = FwdSmem<Boxes, BN, Stages>;
   extern __shared__ char raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kCols = 256;  // S (P over it) in [0, BN), O in [128, 128 + Dh)
+  constexpr int kCols = 256;  // two S buffers (P over them) of BN = 64, O from 128
   const FstGroupedProblem& p = a.prob;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const BlockAt at = block_at(p, blocks);
@@ -69,9 +70,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(smem_addr(&sm.v_full[s]), 1);
       mbar_init(smem_addr(&sm.v_empty[s]), 1);
     }
-    mbar_init(smem_addr(&sm.s_full), 1);
-    mbar_init(smem_addr(&sm.p_ready), 4);
-    mbar_init(smem_addr(&sm.o_full), 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_addr(&sm.s_full[b]), 1);
+      mbar_init(smem_addr(&sm.p_ready[b]), 4);
+      mbar_init(smem_addr(&sm.pv_done[b]), 1);
+    }
     mbar_init_fence();
   }
   tc_fence_before();
@@ -102,28 +105,33 @@ __global__ void __launch_bounds__(kThreads, 2)
   } else if (warp == 5) {
     if (lane == 0) {
       const uint32_t o_instr = instruction<T>((D + 15) & ~15, true, false);
-      ok = mbar_wait(smem_addr(&sm.q_full), 0);
-      for (int it = 0; it < tiles && ok; ++it) {
-        const int s = it % Stages, parity = (it / Stages) & 1;
-        const int steps = (min(BN, end - it * BN) + 15) / 16;  // of 16 keys
-        ok = mbar_wait(smem_addr(&sm.k_full[s]), parity);
-        if (!ok) break;
-        // S may be overwritten: MMAs complete in order, so the product that
-        // read P from it is done before this one writes.
-        product<T, Boxes, kBM, BN>(tS, smem_addr(sm.q), smem_addr(sm.k[s]), D, steps * 16,
-                                   p.scale < 0.f);
-        tc_commit(smem_addr(&sm.s_full));
+      // 16-key steps of a tile.
+      auto steps = [&](int it) { return (min(BN, end - it * BN) + 15) / 16; };
+      // S of a tile. Its buffer may be overwritten: MMAs complete in order,
+      // so the product that read P from it two tiles ago is done by then.
+      auto logits = [&](int it) {
+        const int s = it % Stages;
+        if (!mbar_wait(smem_addr(&sm.k_full[s]), (it / Stages) & 1)) return false;
+        product<T, Boxes, kBM, BN>(tS + it % 2 * BN, smem_addr(sm.q), smem_addr(sm.k[s]), D,
+                                   steps(it) * 16, p.scale < 0.f);
+        tc_commit(smem_addr(&sm.s_full[it % 2]));
         tc_commit(smem_addr(&sm.k_empty[s]));
-        ok = mbar_wait(smem_addr(&sm.v_full[s]), parity) &&
-             mbar_wait(smem_addr(&sm.p_ready), it & 1);
+        return true;
+      };
+      ok = mbar_wait(smem_addr(&sm.q_full), 0) && logits(0) && (tiles == 1 || logits(1));
+      for (int it = 0; it < tiles && ok; ++it) {
+        const int s = it % Stages;
+        ok = mbar_wait(smem_addr(&sm.v_full[s]), (it / Stages) & 1) &&
+             mbar_wait(smem_addr(&sm.p_ready[it % 2]), (it / 2) & 1);
         if (!ok) break;
         tc_fence_after();
-        for (int c = 0; c < steps; ++c)
-          mma_ts(tO, tS + c * 8, operand(smem_addr(sm.v[s]) + c * 2048, BN * 128), o_instr,
-                 it > 0 || c > 0);
+        for (int c = 0; c < steps(it); ++c)
+          mma_ts(tO, tS + it % 2 * BN + c * 8, operand(smem_addr(sm.v[s]) + c * 2048, BN * 128),
+                 o_instr, it > 0 || c > 0);
+        tc_commit(smem_addr(&sm.pv_done[it % 2]));
         tc_commit(smem_addr(&sm.v_empty[s]));
+        if (it + 2 < tiles) ok = logits(it + 2);
       }
-      if (ok) tc_commit(smem_addr(&sm.o_full));
     }
   } else {
     const uint32_t quad = (uint32_t)(warp * 32) << 16;
@@ -137,13 +145,17 @@ __global__ void __launch_bounds__(kThreads, 2)
       // than the tile's keys.
       const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
       const bool edge = j0 + BN > t.len || (p.causal && j0 + BN > t.i0 + 1);
-      ok = mbar_wait(smem_addr(&sm.s_full), it & 1);
+      const uint32_t tSt = tS + quad + it % 2 * BN;
+      ok = mbar_wait(smem_addr(&sm.s_full[it % 2]), (it / 2) & 1);
+      // O += P V of two tiles ago: long done, but waited for, so that the
+      // wait on the last one below can only mean that one.
+      if (ok && it >= 2) ok = mbar_wait(smem_addr(&sm.pv_done[it % 2]), (it / 2 - 1) & 1);
       if (!ok) break;
       tc_fence_after();
       float s[BN / 32][32];
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c)
-        if (c * 32 < nk) tmem_ld32(s[c], tS + quad + c * 32);
+        if (c * 32 < nk) tmem_ld32(s[c], tSt + c * 32);
       tmem_wait_ld();
       float mx = m;
 #pragma unroll
@@ -154,8 +166,17 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e < lim ? s[c][e] : -INFINITY;
         }
+        float part[4] = {mx, s[c][0], s[c][1], s[c][2]};
 #pragma unroll
-        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[c][e]);
+        for (int e = 3; e < 27; e += 8) {
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            part[f] = max3(part[f], s[c][e + 2 * f], s[c][e + 2 * f + 1]);
+        }
+        part[0] = max3(part[0], s[c][27], s[c][28]);
+        part[1] = max3(part[1], s[c][29], s[c][30]);
+        part[2] = max3(part[2], s[c][31], part[3]);
+        mx = max3(part[0], part[1], part[2]);
       }
       // First tile: O is written, not added to, so m may move freely.
       if (it == 0) {
@@ -168,24 +189,31 @@ __global__ void __launch_bounds__(kThreads, 2)
             m = mx;
             l *= keep;
           }
+          ok = mbar_wait(smem_addr(&sm.pv_done[(it - 1) % 2]), ((it - 1) / 2) & 1);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll 1
           for (int d = 0; d < D; d += 16) tmem_scale16(tO + quad + d, keep);
         }
       }
       const float off = m == -INFINITY ? 0.f : m * c2;
-      float sum = 0.f;
+      const pair_t scale2 = pair(c2, c2), off2 = pair(-off, -off);
+      pair_t sums = pair(0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c) {
         if (c * 32 >= nk) continue;
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float x = ex2(fmaf(s[c][e], c2, -off)), y = ex2(fmaf(s[c][e + 1], c2, -off));
-          sum += x + y;
-          w[e / 2] = Elem<T>::pack(x, y);
+          float2 x = split(fma2(pair(s[c][e], s[c][e + 1]), scale2, off2));
+          x.x = ex2(x.x);
+          x.y = ex2(x.y);
+          sums = add2(sums, pair(x.x, x.y));
+          w[e / 2] = Elem<T>::pack(x.x, x.y);
         }
-        tmem_st16(tS + quad + c * 16, w);
+        tmem_st16(tSt + c * 16, w);
       }
+      const float sum = split(sums).x + split(sums).y;
       l += sum;
       if (nk & 15) {
         // Keys up to the next multiple of 16 have p = 0, but what V holds
@@ -198,9 +226,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&sm.p_ready));
+      if (lane == 0) mbar_arrive(smem_addr(&sm.p_ready[it % 2]));
     }
-    if (ok) ok = mbar_wait(smem_addr(&sm.o_full), 0);
+    if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(tiles - 1) % 2]), ((tiles - 1) / 2) & 1);
     tc_fence_after();
     const bool live = i < t.len;
     store_row<T>(live ? row_ptr<T>(a.out, t, at.h, i) : nullptr, tO + quad, D,
@@ -236,8 +264,8 @@ int launch(const FstGroupedForwardArgs& a, cudaStream_t st) {
 
 template <typename T>
 int launch_t(const FstGroupedForwardArgs& a, cudaStream_t st) {
-  if (a.prob.head_dim <= 64) return launch<T, 1, 128, 2>(a, st);
-  return launch<T, 2, 128, 1>(a, st);
+  if (a.prob.head_dim <= 64) return launch<T, 1, 64, 3>(a, st);
+  return launch<T, 2, 64, 2>(a, st);
 }
 
 }  // namespace
