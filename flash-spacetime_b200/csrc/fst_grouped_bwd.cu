@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   constexpr int kCols = 256;  // S (dS over it) 0, dP 64, dQ 128
   const FstGroupedProblem& p = a.prob;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const BlockAt at = block_at(p, blocks);
   RowTile t;
   if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
@@ -98,28 +98,28 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       }
     }
   } else if (warp == 5) {
-    if (lane == 0) {
-      const uint32_t acc_instr = instruction<T>((D + 15) & ~15, true, false);
-      ok = mbar_wait(smem_addr(&sm.own_full), 0);
-      for (int it = 0; it < tiles && ok; ++it) {
-        const int s = it % Stages;
-        const int steps = (min(kBN, end - it * kBN) + 15) / 16;
-        ok = mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1);
-        if (!ok) break;
-        product<T, Boxes, kBM, kBN>(tS, smem_addr(sm.q), smem_addr(sm.k[s]), D, steps * 16,
-                                    p.scale < 0.f);
-        product<T, Boxes, kBM, kBN>(tP, smem_addr(sm.g), smem_addr(sm.v[s]), D, steps * 16, false);
-        tc_commit(smem_addr(&sm.s_full));
-        ok = mbar_wait(smem_addr(&sm.ready), it & 1);
-        if (!ok) break;
-        tc_fence_after();
-        for (int c = 0; c < steps; ++c)
-          mma_ts(tQ, tS + c * 8, operand(smem_addr(sm.k[s]) + c * 2048, kBN * 128), acc_instr,
-                 it > 0 || c > 0);
-        tc_commit(smem_addr(&sm.empty[s]));
-      }
-      if (ok) tc_commit(smem_addr(&sm.done));
+    const uint32_t leader = elect_one();
+    const int n = uniform(tiles), last = uniform(end), dim = uniform(D);
+    const uint32_t s_mem = uniform(tS);
+    const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
+    ok = mbar_wait(smem_addr(&sm.own_full), 0);
+    for (int it = 0; it < n && ok; ++it) {
+      const int s = it % Stages;
+      const int keys = min(kBN, last - it * kBN), up = (keys + 15) & ~15;
+      ok = mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1);
+      if (!ok) break;
+      product<T, Boxes, kBM, kBN>(s_mem, smem_addr(sm.q), smem_addr(sm.k[s]), dim, up,
+                                  p.scale < 0.f, leader);
+      product<T, Boxes, kBM, kBN>(s_mem + 64, smem_addr(sm.g), smem_addr(sm.v[s]), dim, up, false,
+                                  leader);
+      tc_commit(smem_addr(&sm.s_full), leader);
+      ok = mbar_wait(smem_addr(&sm.ready), it & 1);
+      if (!ok) break;
+      tc_fence_after();
+      accumulate<kBN>(s_mem + 128, s_mem, smem_addr(sm.k[s]), keys, acc_instr, it > 0, leader);
+      tc_commit(smem_addr(&sm.empty[s]), leader);
     }
+    if (ok) tc_commit(smem_addr(&sm.done), leader);
   } else {
     const uint32_t quad = (uint32_t)(warp * 32) << 16;
     const int i = t.i0 + warp * 32 + lane;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
   constexpr int kCols = Groups * 128 + 2 * kAcc;      // 256 or 512
   constexpr int kTma = Groups * 4, kMma = kTma + 1;   // warps
   const FstGroupedProblem& p = a.prob;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int kh = blockIdx.x / blocks, id = blockIdx.x - kh * blocks;
   const int group = p.heads / p.kv_heads;
   RowTile t;
@@ -289,39 +289,38 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
       }
     }
   } else if (warp == kMma) {
-    if (lane == 0) {
-      const uint32_t acc_instr = instruction<T>((D + 15) & ~15, true, false);
-      auto rows_of = [&](int it) { return min(kBN, t.len - first - it % per_head * kBN); };
-      // S^T and dP^T of a tile into its group's accumulators. The MMAs run in
-      // order, so those that read the tile before from there are done.
-      auto logits = [&](int it) {
-        const int s = it % Stages, w = it % Groups, n = (rows_of(it) + 15) & ~15;
-        if (!mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1)) return false;
-        product<T, Boxes, kBM, kBN>(tmem + w * 128, smem_addr(sm.k), smem_addr(sm.q[s]), D, n,
-                                    p.scale < 0.f);
-        product<T, Boxes, kBM, kBN>(tmem + w * 128 + 64, smem_addr(sm.v), smem_addr(sm.g[s]), D,
-                                    n, false);
-        tc_commit(smem_addr(&sm.s_full[w]));
-        return true;
-      };
-      ok = mbar_wait(smem_addr(&sm.own_full), 0);
-      for (int it = 0; it < Groups && it < tiles && ok; ++it) ok = logits(it);
-      for (int it = 0; it < tiles && ok; ++it) {
-        const int s = it % Stages, w = it % Groups, steps = (rows_of(it) + 15) / 16;
-        ok = mbar_wait(smem_addr(&sm.ready[w]), (it / Groups) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        for (int c = 0; c < steps; ++c)
-          mma_ts(tV, tmem + w * 128 + c * 8, operand(smem_addr(sm.g[s]) + c * 2048, kBN * 128),
-                 acc_instr, it > 0 || c > 0);
-        for (int c = 0; c < steps; ++c)
-          mma_ts(tK, tmem + w * 128 + 64 + c * 8,
-                 operand(smem_addr(sm.q[s]) + c * 2048, kBN * 128), acc_instr, it > 0 || c > 0);
-        tc_commit(smem_addr(&sm.empty[s]));
-        if (it + Groups < tiles) ok = logits(it + Groups);
-      }
-      if (ok) tc_commit(smem_addr(&sm.done));
+    const uint32_t leader = elect_one();
+    const int n = uniform(tiles), each = uniform(per_head), rows = uniform(t.len - first);
+    const int dim = uniform(D);
+    const uint32_t mem = uniform(tmem), v_mem = mem + Groups * 128, k_mem = v_mem + kAcc;
+    const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
+    auto rows_of = [&](int it) { return min(kBN, rows - it % each * kBN); };
+    // S^T and dP^T of a tile into its group's accumulators. The MMAs run in
+    // order, so those that read the tile before from there are done.
+    auto logits = [&](int it) {
+      const int s = it % Stages, w = it % Groups, up = (rows_of(it) + 15) & ~15;
+      if (!mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1)) return false;
+      product<T, Boxes, kBM, kBN>(mem + w * 128, smem_addr(sm.k), smem_addr(sm.q[s]), dim, up,
+                                  p.scale < 0.f, leader);
+      product<T, Boxes, kBM, kBN>(mem + w * 128 + 64, smem_addr(sm.v), smem_addr(sm.g[s]), dim,
+                                  up, false, leader);
+      tc_commit(smem_addr(&sm.s_full[w]), leader);
+      return true;
+    };
+    ok = mbar_wait(smem_addr(&sm.own_full), 0);
+    for (int it = 0; it < Groups && it < n && ok; ++it) ok = logits(it);
+    for (int it = 0; it < n && ok; ++it) {
+      const int s = it % Stages, w = it % Groups, q_rows = rows_of(it);
+      ok = mbar_wait(smem_addr(&sm.ready[w]), (it / Groups) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      accumulate<kBN>(v_mem, mem + w * 128, smem_addr(sm.g[s]), q_rows, acc_instr, it > 0, leader);
+      accumulate<kBN>(k_mem, mem + w * 128 + 64, smem_addr(sm.q[s]), q_rows, acc_instr, it > 0,
+                      leader);
+      tc_commit(smem_addr(&sm.empty[s]), leader);
+      if (it + Groups < n) ok = logits(it + Groups);
     }
+    if (ok) tc_commit(smem_addr(&sm.done), leader);
   } else {
     const int w = warp / 4;
     const uint32_t quad = (uint32_t)(warp % 4 * 32) << 16;

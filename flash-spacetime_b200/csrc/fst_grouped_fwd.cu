@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   constexpr int kCols = 256;  // two S buffers (P over them) of BN = 64, O from 128
   const FstGroupedProblem& p = a.prob;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const BlockAt at = block_at(p, blocks);
   RowTile t;
   if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
@@ -103,35 +103,34 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   } else if (warp == 5) {
-    if (lane == 0) {
-      const uint32_t o_instr = instruction<T>((D + 15) & ~15, true, false);
-      // 16-key steps of a tile.
-      auto steps = [&](int it) { return (min(BN, end - it * BN) + 15) / 16; };
-      // S of a tile. Its buffer may be overwritten: MMAs complete in order,
-      // so the product that read P from it two tiles ago is done by then.
-      auto logits = [&](int it) {
-        const int s = it % Stages;
-        if (!mbar_wait(smem_addr(&sm.k_full[s]), (it / Stages) & 1)) return false;
-        product<T, Boxes, kBM, BN>(tS + it % 2 * BN, smem_addr(sm.q), smem_addr(sm.k[s]), D,
-                                   steps(it) * 16, p.scale < 0.f);
-        tc_commit(smem_addr(&sm.s_full[it % 2]));
-        tc_commit(smem_addr(&sm.k_empty[s]));
-        return true;
-      };
-      ok = mbar_wait(smem_addr(&sm.q_full), 0) && logits(0) && (tiles == 1 || logits(1));
-      for (int it = 0; it < tiles && ok; ++it) {
-        const int s = it % Stages;
-        ok = mbar_wait(smem_addr(&sm.v_full[s]), (it / Stages) & 1) &&
-             mbar_wait(smem_addr(&sm.p_ready[it % 2]), (it / 2) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        for (int c = 0; c < steps(it); ++c)
-          mma_ts(tO, tS + it % 2 * BN + c * 8, operand(smem_addr(sm.v[s]) + c * 2048, BN * 128),
-                 o_instr, it > 0 || c > 0);
-        tc_commit(smem_addr(&sm.pv_done[it % 2]));
-        tc_commit(smem_addr(&sm.v_empty[s]));
-        if (it + 2 < tiles) ok = logits(it + 2);
-      }
+    const uint32_t leader = elect_one();
+    const int n = uniform(tiles), last = uniform(end), dim = uniform(D);
+    const uint32_t s_mem = uniform(tS), o_mem = s_mem + 128;
+    const uint32_t o_instr = instruction<T>((dim + 15) & ~15, true, false);
+    auto keys = [&](int it) { return min(BN, last - it * BN); };
+    // S of a tile. Its buffer may be overwritten: MMAs complete in order,
+    // so the product that read P from it two tiles ago is done by then.
+    auto logits = [&](int it) {
+      const int s = it % Stages;
+      if (!mbar_wait(smem_addr(&sm.k_full[s]), (it / Stages) & 1)) return false;
+      product<T, Boxes, kBM, BN>(s_mem + it % 2 * BN, smem_addr(sm.q), smem_addr(sm.k[s]), dim,
+                                 (keys(it) + 15) & ~15, p.scale < 0.f, leader);
+      tc_commit(smem_addr(&sm.s_full[it % 2]), leader);
+      tc_commit(smem_addr(&sm.k_empty[s]), leader);
+      return true;
+    };
+    ok = mbar_wait(smem_addr(&sm.q_full), 0) && logits(0) && (n == 1 || logits(1));
+    for (int it = 0; it < n && ok; ++it) {
+      const int s = it % Stages;
+      ok = mbar_wait(smem_addr(&sm.v_full[s]), (it / Stages) & 1) &&
+           mbar_wait(smem_addr(&sm.p_ready[it % 2]), (it / 2) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      accumulate<BN>(o_mem, s_mem + it % 2 * BN, smem_addr(sm.v[s]), keys(it), o_instr, it > 0,
+                     leader);
+      tc_commit(smem_addr(&sm.pv_done[it % 2]), leader);
+      tc_commit(smem_addr(&sm.v_empty[s]), leader);
+      if (it + 2 < n) ok = logits(it + 2);
     }
   } else {
     const uint32_t quad = (uint32_t)(warp * 32) << 16;

@@ -59,10 +59,28 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// Arrives on `bar` when every MMA this thread has issued so far is complete.
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t leader;
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(leader));
+  return leader;
+}
+// A value that is the same in every lane, in a form the compiler knows to be.
+// The issuing warp runs converged, on such values, and leaves the choice of
+// the issuing lane to a predicate on each instruction: descriptors are then
+// formed on the uniform datapath (a lane's branch of its own costs about 100
+// cycles an MMA to move them there).
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// Arrives on `bar` when every MMA the leader has issued so far is complete.
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(
+          bar),
+      "r"(leader)
       : "memory");
 }
 
@@ -83,19 +101,19 @@ __device__ __forceinline__ uint32_t instruction(int n, bool b_mn_major, bool neg
          (b_mn_major ? 1u << 16 : 0) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
+                                       bool add, uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((int)add)
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((int)add), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
+                                       bool add, uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((int)add)
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((int)add), "r"(leader)
       : "memory");
 }
 
@@ -226,13 +244,24 @@ __device__ __forceinline__ void zero_tile_rows(char* tile, int first, int last, 
 // d[128][n] = A B^T over the D channels, both tiles K-major in shared memory.
 template <typename T, int Boxes, int ARows, int BRows>
 __device__ __forceinline__ void product(uint32_t d, uint32_t A, uint32_t B, int D, int n,
-                                        bool negate) {
+                                        bool negate, uint32_t leader) {
   const uint32_t instr = instruction<T>(n, false, negate);
+  const uint64_t a = operand(A, 0), b = operand(B, 0);
 #pragma unroll
   for (int c = 0; c < Boxes * 4; ++c)
     if (c * 16 < D)
-      mma_ss(d, operand(A + (c / 4) * ARows * 128 + (c % 4) * 32, 0),
-             operand(B + (c / 4) * BRows * 128 + (c % 4) * 32, 0), instr, c > 0);
+      mma_ss(d, a + ((c / 4) * ARows * 128 + (c % 4) * 32) / 16,
+             b + ((c / 4) * BRows * 128 + (c % 4) * 32) / 16, instr, c > 0, leader);
+}
+// d[128][n] (+)= P X over `rows` rows (rounded up to 16) of X, a tile of BRows
+// rows; P 16-bit values in tensor memory.
+template <int BRows>
+__device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, int rows,
+                                           uint32_t instr, bool add, uint32_t leader) {
+  const uint64_t x = operand(X, BRows * 128);
+#pragma unroll
+  for (int c = 0; c < BRows / 16; ++c)
+    if (c * 16 < rows) mma_ts(d, P + c * 8, x + c * 2048 / 16, instr, add || c > 0, leader);
 }
 
 // The block's rows of no event: zeros, in 16-byte vectors, by n threads.
