@@ -109,7 +109,7 @@ int fst_grouped_backward(const FstGroupedBackwardArgs* a, void* stream) {
   if (rc) return rc;
   if (a->prob.total_rows == 0) return FST_OK;
   if (any_null({a->q.data, a->k.data, a->v.data, a->out.data, a->dout.data, a->dq.data,
-                a->dk.data, a->dv.data, a->lse, a->delta}))
+                a->dk.data, a->dv.data, a->lse, a->stats}))
     return api_fail(FST_ERR_INVALID, "grouped backward: a required pointer is null");
   cudaGetLastError();
   const cudaStream_t st = (cudaStream_t)stream;

@@ -3,11 +3,11 @@
 // atomics and are the same bits on every run.
 //
 // Row kernel (dq, and D_i = dO_i . o_i): a block owns 128 query rows of a head
-// and walks the keys in tiles of 64:
+// and walks the keys:
 //   S = Q K^T, dP = dO V^T  ->  dS = P (dP - D)  ->  dQ += dS K.
 // Column kernel (dk, dv): a block owns 128 keys and walks the query rows, and
-// the heads of the group, in tiles of 64, with the products transposed so
-// that a thread owns a key:
+// the heads of the group, with the products transposed so that a thread owns
+// a key:
 //   S^T = K Q^T, dP^T = V dO^T  ->  dV += P^T dO, dK += dS^T Q.
 // P and dS are written over S and dP in tensor memory as 16-bit values and are
 // the A operands of the second products; each is rounded once to the type.
@@ -16,6 +16,16 @@
 // seven products and one exponential more than a single pass would take, and
 // saves its fp32 additions into dq in memory, whose order would change with
 // the schedule.
+//
+// A tile goes through the tensor cores in two halves, so that they and the
+// exponentials work at the same time on one pair of accumulators:
+//   rows:     S of the next tile | dS of this one;  dQ, next dP | next P
+//   columns:  dV, next S         | dS of this one;  dK, next dP | next P
+// W warpgroups share a tile of 64 W rows of the other side, 64 columns each.
+// Up to Dh = 64 one group and 256 columns of tensor memory: two blocks an SM.
+// Above, dV and dK (or dQ) need twice the columns; two groups and one block,
+// whose products are 128 wide: a product of two shared-memory operands reads
+// 4 KB of A per 16 channels whatever its width, which bounds 64 wide ones.
 
 #include <cuda_runtime.h>
 
@@ -28,101 +38,121 @@ namespace grouped {
 namespace {
 
 constexpr int kBM = 128;  // rows a block owns
-constexpr int kBN = 64;   // rows of the other side per tile
+constexpr int threads_of(int W) { return W * 128 + 64; }
+constexpr int resident_of(int W) { return W == 1 ? 2 : 1; }
 
 // ---- dq ---------------------------------------------------------------------
 
-template <int Boxes, int Stages>
+template <int Boxes, int W, int Stages>
 struct RowSmem {
   alignas(1024) char q[Boxes * kBM * 128];
   alignas(1024) char g[Boxes * kBM * 128];
-  alignas(1024) char k[Stages][Boxes * kBN * 128];
-  alignas(1024) char v[Stages][Boxes * kBN * 128];
-  uint64_t own_full, full[Stages], empty[Stages], s_full, ready, done;
+  alignas(1024) char k[Stages][Boxes * W * 64 * 128];
+  alignas(1024) char v[Stages][Boxes * W * 64 * 128];
+  uint64_t own_full, full[Stages], empty[Stages], s_full, s_free, dp_full, ds_ready, done;
   uint32_t tmem;
 };
 
-constexpr int kRowThreads = 192;
-
-template <typename T, int Boxes, int Stages>
-__global__ void __launch_bounds__(kRowThreads, 2)
-    dq_kernel(const __grid_constant__ TileMaps maps, const FstGroupedBackwardArgs a, int blocks) {
-  using Smem = RowSmem<Boxes, Stages>;
+template <typename T, int Boxes, int W, int Stages>
+__global__ void __launch_bounds__(threads_of(W), resident_of(W))
+    dq_kernel(const __grid_constant__ TileMaps maps, const FstGroupedBackwardArgs a, int blocks,
+              float* stats) {
+  using Smem = RowSmem<Boxes, W, Stages>;
   extern __shared__ char raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kCols = 256;  // S (dS over it) 0, dP 64, dQ 128
+  constexpr int kBN = W * 64, kCols = W * 256, kTma = W * 4, kMma = kTma + 1;
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const BlockAt at = block_at(p, blocks);
   RowTile t;
   if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
   const int D = p.head_dim;
-  zero_dead_rows<T, kBM>(a.dq, t, at.h, D, kRowThreads);
+  zero_dead_rows<T, kBM>(a.dq, t, at.h, D, threads_of(W));
   if (t.i0 >= t.len) return;
   const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
   const int tiles = (end + kBN - 1) / kBN;
 
-  if (warp == 4) {
-    tmem_alloc<kCols>(smem_addr(&sm.tmem));
-  } else if (threadIdx.x == 0) {
+  auto load = [&](int it) {
+    const int s = it % Stages;
+    const uint32_t full = smem_addr(&sm.full[s]);
+    mbar_arrive_tx(full, 2 * Boxes * kBN * 128);
+    load_boxes<Boxes, kBN>(smem_addr(sm.k[s]), &maps.k, full, t.base + it * kBN, at.kh, t.ev);
+    load_boxes<Boxes, kBN>(smem_addr(sm.v[s]), &maps.v, full, t.base + it * kBN, at.kh, t.ev);
+  };
+  if (warp == kTma && lane == 0) {
     mbar_init(smem_addr(&sm.own_full), 1);
     for (int s = 0; s < Stages; ++s) {
       mbar_init(smem_addr(&sm.full[s]), 1);
       mbar_init(smem_addr(&sm.empty[s]), 1);
     }
     mbar_init(smem_addr(&sm.s_full), 1);
-    mbar_init(smem_addr(&sm.ready), 4);
+    mbar_init(smem_addr(&sm.s_free), W * 4);
+    mbar_init(smem_addr(&sm.dp_full), 1);
+    mbar_init(smem_addr(&sm.ds_ready), W * 4);
     mbar_init(smem_addr(&sm.done), 1);
     mbar_init_fence();
+    // The first tiles set out before the others are ready for them.
+    const uint32_t own = smem_addr(&sm.own_full);
+    mbar_arrive_tx(own, 2 * Boxes * kBM * 128);
+    load_boxes<Boxes, kBM>(smem_addr(sm.q), &maps.q, own, t.base + t.i0, at.h, t.ev);
+    load_boxes<Boxes, kBM>(smem_addr(sm.g), &maps.g, own, t.base + t.i0, at.h, t.ev);
+    for (int it = 0; it < Stages && it < tiles; ++it) load(it);
   }
+  if (warp == kMma) tmem_alloc<kCols>(smem_addr(&sm.tmem));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tS = sm.tmem, tP = tS + 64, tQ = tS + 128;
+  const uint32_t tmem = sm.tmem;  // S, dP (dS over it), dQ
 
   bool ok = true;
-  if (warp == 4) {
+  if (warp == kTma) {
     if (lane == 0) {
-      const uint32_t own = smem_addr(&sm.own_full);
-      mbar_arrive_tx(own, 2 * Boxes * kBM * 128);
-      load_boxes<Boxes, kBM>(smem_addr(sm.q), &maps.q, own, t.base + t.i0, at.h, t.ev);
-      load_boxes<Boxes, kBM>(smem_addr(sm.g), &maps.g, own, t.base + t.i0, at.h, t.ev);
-      for (int it = 0; it < tiles; ++it) {
-        const int s = it % Stages, round = it / Stages;
-        if (round) ok = mbar_wait(smem_addr(&sm.empty[s]), (round - 1) & 1);
-        if (!ok) break;
-        const uint32_t full = smem_addr(&sm.full[s]);
-        mbar_arrive_tx(full, 2 * Boxes * kBN * 128);
-        load_boxes<Boxes, kBN>(smem_addr(sm.k[s]), &maps.k, full, t.base + it * kBN, at.kh, t.ev);
-        load_boxes<Boxes, kBN>(smem_addr(sm.v[s]), &maps.v, full, t.base + it * kBN, at.kh, t.ev);
+      for (int it = Stages; it < tiles && ok; ++it) {
+        ok = mbar_wait(smem_addr(&sm.empty[it % Stages]), (it / Stages - 1) & 1);
+        if (ok) load(it);
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == kMma) {
     const uint32_t leader = elect_one();
     const int n = uniform(tiles), last = uniform(end), dim = uniform(D);
-    const uint32_t s_mem = uniform(tS);
+    const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, q_mem = p_mem + kBN;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
-    ok = mbar_wait(smem_addr(&sm.own_full), 0);
-    for (int it = 0; it < n && ok; ++it) {
-      const int s = it % Stages;
-      const int keys = min(kBN, last - it * kBN), up = (keys + 15) & ~15;
-      ok = mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1);
-      if (!ok) break;
-      product<T, Boxes, kBM, kBN>(s_mem, smem_addr(sm.q), smem_addr(sm.k[s]), dim, up,
-                                  p.scale < 0.f, leader);
-      product<T, Boxes, kBM, kBN>(s_mem + 64, smem_addr(sm.g), smem_addr(sm.v[s]), dim, up, false,
-                                  leader);
+    auto keys = [&](int it) { return min(kBN, last - it * kBN); };
+    auto logits = [&](int it) {
+      if (!mbar_wait(smem_addr(&sm.full[it % Stages]), (it / Stages) & 1)) return false;
+      product<T, Boxes, kBM, kBN>(s_mem, smem_addr(sm.q), smem_addr(sm.k[it % Stages]), dim,
+                                  (keys(it) + 15) & ~15, p.scale < 0.f, leader);
       tc_commit(smem_addr(&sm.s_full), leader);
-      ok = mbar_wait(smem_addr(&sm.ready), it & 1);
+      return true;
+    };
+    // Over dS: MMAs complete in order, so the product that read it is done.
+    auto weights = [&](int it) {
+      product<T, Boxes, kBM, kBN>(p_mem, smem_addr(sm.g), smem_addr(sm.v[it % Stages]), dim,
+                                  (keys(it) + 15) & ~15, false, leader);
+      tc_commit(smem_addr(&sm.dp_full), leader);
+    };
+    ok = mbar_wait(smem_addr(&sm.own_full), 0) && logits(0);
+    if (ok) weights(0);
+    for (int it = 0; it < n && ok; ++it) {
+      if (it + 1 < n) {
+        ok = mbar_wait(smem_addr(&sm.s_free), it & 1);
+        tc_fence_after();
+        ok = ok && logits(it + 1);
+      }
+      ok = ok && mbar_wait(smem_addr(&sm.ds_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
-      accumulate<kBN>(s_mem + 128, s_mem, smem_addr(sm.k[s]), keys, acc_instr, it > 0, leader);
-      tc_commit(smem_addr(&sm.empty[s]), leader);
+      accumulate<kBN>(q_mem, p_mem, smem_addr(sm.k[it % Stages]), keys(it), acc_instr, it > 0,
+                      leader);
+      tc_commit(smem_addr(&sm.empty[it % Stages]), leader);
+      if (it + 1 < n) weights(it + 1);
     }
     if (ok) tc_commit(smem_addr(&sm.done), leader);
   } else {
-    const uint32_t quad = (uint32_t)(warp * 32) << 16;
-    const int i = t.i0 + warp * 32 + lane;
+    const int w = warp / 4, row = warp % 4 * 32 + lane;  // key columns [64 w, +64) of a tile
+    const uint32_t quad = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t tS = tmem + quad + w * 64, tP = tS + kBN;
+    const int i = t.i0 + row;
     const bool live = i < t.len;
     const float c2 = fabsf(p.scale) * kLog2e;
     float lse2 = 0.f, delta = 0.f;
@@ -138,87 +168,109 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       }
       const int64_t st = stat_at(p, t, p.heads, at.h, i);
       lse2 = a.lse[st] * kLog2e;
-      a.delta[st] = delta;
+      if (w == 0) {  // for the column kernel, in the form it adds them
+        stats[st] = -lse2;
+        stats[st + p.total_rows * p.heads] = -delta;
+      }
     }
     const pair_t scale2 = pair(c2, c2), lse2n = pair(-lse2, -lse2), delta2n = pair(-delta, -delta);
     for (int it = 0; it < tiles; ++it) {
-      const int j0 = it * kBN, nk = min(kBN, end - j0);
+      const int j0 = it * kBN + w * 64, nk = end - j0;
       const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
-      const bool edge = j0 + kBN > t.len || (p.causal && j0 + kBN > t.i0 + 1);
+      const bool edge = j0 + 64 > t.len || (p.causal && j0 + 64 > t.i0 + 1);
       ok = mbar_wait(smem_addr(&sm.s_full), it & 1);
       if (!ok) break;
       tc_fence_after();
+      float s[2][32];
 #pragma unroll
-      for (int c = 0; c < kBN / 32; ++c) {
-        if (c * 32 >= nk) continue;
-        float s[32], dp[32];
-        tmem_ld32(s, tS + quad + c * 32);
-        tmem_ld32(dp, tP + quad + c * 32);
-        tmem_wait_ld();
-        pin(s);
-        pin(dp);
-        uint32_t w[16];
+      for (int c = 0; c < 2; ++c)
+        if (c * 32 < nk) tmem_ld32(s[c], tS + c * 32);
+      tmem_wait_ld();
+      pin(s[0]);
+      pin(s[1]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&sm.s_free));
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          float2 x = split(fma2(pair(s[e], s[e + 1]), scale2, lse2n));
-          x = split(mul2(pair(ex2(x.x), ex2(x.y)), add2(pair(dp[e], dp[e + 1]), delta2n)));
-          s[e] = x.x;
-          s[e + 1] = x.y;
+          const float2 x = split(fma2(pair(s[c][e], s[c][e + 1]), scale2, lse2n));
+          s[c][e] = ex2(x.x);
+          s[c][e + 1] = ex2(x.y);
+        }
+      ok = mbar_wait(smem_addr(&sm.dp_full), it & 1);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (c * 32 >= nk) continue;
+        float dp[32];
+        tmem_ld32(dp, tP + c * 32);
+        tmem_wait_ld();
+        pin(dp);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = split(
+              mul2(pair(s[c][e], s[c][e + 1]), add2(pair(dp[e], dp[e + 1]), delta2n)));
+          dp[e] = x.x;
+          dp[e + 1] = x.y;
         }
         if (edge) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = c * 32 + e < lim ? s[e] : 0.f;
+          for (int e = 0; e < 32; ++e) dp[e] = c * 32 + e < lim ? dp[e] : 0.f;
         }
+        uint32_t x[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = Elem<T>::pack(s[2 * e], s[2 * e + 1]);
-        tmem_st16(tS + quad + c * 16, w);
+        for (int e = 0; e < 16; ++e) x[e] = Elem<T>::pack(dp[2 * e], dp[2 * e + 1]);
+        tmem_st16(tP + c * 16, x);
       }
-      if (nk & 15)  // dS is 0 there, and must not meet another event's NaN
-        zero_tile_rows<Boxes, kBN>(sm.k[it % Stages], nk, (nk + 15) & ~15, threadIdx.x, 128);
+      const int all = min(kBN, end - it * kBN);
+      if (all & 15)  // dS is 0 there, and must not meet another event's NaN
+        zero_tile_rows<Boxes, kBN>(sm.k[it % Stages], all, (all + 15) & ~15, threadIdx.x, W * 128);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&sm.ready));
+      if (lane == 0) mbar_arrive(smem_addr(&sm.ds_ready));
     }
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
-    store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) : nullptr, tQ + quad, D,
+    // The groups share the columns of the result.
+    store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr,
+                 tmem + quad + 2 * kBN + w * 64, W == 1 ? D : min(D - w * 64, 64),
                  ok ? p.scale : NAN);
     tc_fence_before();
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == 4) tmem_free<kCols>(tS);
+  if (warp == kMma) tmem_free<kCols>(tmem);
 }
 
 // ---- dk, dv -----------------------------------------------------------------
 
-// Groups: warpgroups of the block that turn S^T and dP^T into P^T and dS^T, on
-// alternate tiles, each with its own pair of accumulators.
-template <int Boxes, int Stages, int Groups>
+template <int Boxes, int W, int Stages>
 struct ColSmem {
   alignas(1024) char k[Boxes * kBM * 128];
   alignas(1024) char v[Boxes * kBM * 128];
-  alignas(1024) char q[Stages][Boxes * kBN * 128];
-  alignas(1024) char g[Stages][Boxes * kBN * 128];
-  alignas(16) float lse2n[Stages][kBN];   // -log2(e) lse of the query rows
-  alignas(16) float deltan[Stages][kBN];  // -D
-  uint64_t own_full, full[Stages], empty[Stages], s_full[Groups], ready[Groups], done;
+  alignas(1024) char q[Stages][Boxes * W * 64 * 128];
+  alignas(1024) char g[Stages][Boxes * W * 64 * 128];
+  alignas(16) float lse2n[Stages][W * 64];   // -log2(e) lse of the query rows
+  alignas(16) float deltan[Stages][W * 64];  // -D
+  uint64_t own_full, full[Stages], empty[Stages], s_full, p_ready, dp_full, ds_ready, done;
   uint32_t tmem;
 };
 
-constexpr int col_threads(int groups) { return groups * 128 + 64; }
-
-template <typename T, int Boxes, int Stages, int Groups>
-__global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
-    dkv_kernel(const __grid_constant__ TileMaps maps, const FstGroupedBackwardArgs a, int blocks) {
-  using Smem = ColSmem<Boxes, Stages, Groups>;
+template <typename T, int Boxes, int W, int Stages>
+__global__ void __launch_bounds__(threads_of(W), resident_of(W))
+    dkv_kernel(const __grid_constant__ TileMaps maps, const FstGroupedBackwardArgs a, int blocks,
+               const float* stats) {
+  using Smem = ColSmem<Boxes, W, Stages>;
   extern __shared__ char raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kThreads = col_threads(Groups);
-  constexpr int kAcc = Boxes * 64;                    // columns of dV and of dK
-  constexpr int kCols = Groups * 128 + 2 * kAcc;      // 256 or 512
-  constexpr int kTma = Groups * 4, kMma = kTma + 1;   // warps
+  constexpr int kBN = W * 64, kAcc = Boxes * 64;  // query rows a tile; columns of dV and of dK
+  constexpr int kCols = 2 * kBN + 2 * kAcc;       // 256 or 512
+  constexpr int kTma = W * 4, kMma = kTma + 1;    // warps
+  static_assert(kCols == 256 || kCols == 512, "tensor memory comes in powers of two");
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int kh = blockIdx.x / blocks, id = blockIdx.x - kh * blocks;
@@ -226,42 +278,38 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
   RowTile t;
   if (!find_tile<kBM>(p, id, false, t)) return;
   const int D = p.head_dim;
-  zero_dead_rows<T, kBM>(a.dk, t, kh, D, kThreads);
-  zero_dead_rows<T, kBM>(a.dv, t, kh, D, kThreads);
+  zero_dead_rows<T, kBM>(a.dk, t, kh, D, threads_of(W));
+  zero_dead_rows<T, kBM>(a.dv, t, kh, D, threads_of(W));
   if (t.i0 >= t.len) return;
-  const int first = p.causal ? t.i0 : 0;                    // first query row
-  const int per_head = (t.len - first + kBN - 1) / kBN;     // query tiles a head
+  const int first = p.causal ? t.i0 : 0;                 // first query row
+  const int per_head = (t.len - first + kBN - 1) / kBN;  // query tiles a head
   const int tiles = per_head * group;
 
-  if (warp == kTma) {
-    tmem_alloc<kCols>(smem_addr(&sm.tmem));
-  } else if (threadIdx.x == 0) {
+  if (warp == kTma && lane == 0) {
     mbar_init(smem_addr(&sm.own_full), 1);
     for (int s = 0; s < Stages; ++s) {
-      mbar_init(smem_addr(&sm.full[s]), 2);
+      mbar_init(smem_addr(&sm.full[s]), 1 + 32);  // TMA, and each lane's copies
       mbar_init(smem_addr(&sm.empty[s]), 1);
     }
-    for (int w = 0; w < Groups; ++w) {
-      mbar_init(smem_addr(&sm.s_full[w]), 1);
-      mbar_init(smem_addr(&sm.ready[w]), 4);
-    }
+    mbar_init(smem_addr(&sm.s_full), 1);
+    mbar_init(smem_addr(&sm.p_ready), W * 4);
+    mbar_init(smem_addr(&sm.dp_full), 1);
+    mbar_init(smem_addr(&sm.ds_ready), W * 4);
     mbar_init(smem_addr(&sm.done), 1);
     mbar_init_fence();
+    const uint32_t own = smem_addr(&sm.own_full);
+    mbar_arrive_tx(own, 2 * Boxes * kBM * 128);
+    load_boxes<Boxes, kBM>(smem_addr(sm.k), &maps.k, own, t.base + t.i0, kh, t.ev);
+    load_boxes<Boxes, kBM>(smem_addr(sm.v), &maps.v, own, t.base + t.i0, kh, t.ev);
   }
+  if (warp == kMma) tmem_alloc<kCols>(smem_addr(&sm.tmem));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // Per group S^T and dP^T of 64 columns, then dV, dK.
-  const uint32_t tmem = sm.tmem, tV = tmem + Groups * 128, tK = tV + kAcc;
+  const uint32_t tmem = sm.tmem;  // S^T (P^T over it), dP^T (dS^T over it), dV, dK
 
   bool ok = true;
   if (warp == kTma) {
-    if (lane == 0) {
-      const uint32_t own = smem_addr(&sm.own_full);
-      mbar_arrive_tx(own, 2 * Boxes * kBM * 128);
-      load_boxes<Boxes, kBM>(smem_addr(sm.k), &maps.k, own, t.base + t.i0, kh, t.ev);
-      load_boxes<Boxes, kBM>(smem_addr(sm.v), &maps.v, own, t.base + t.i0, kh, t.ev);
-    }
     int h = kh * group, q0 = first;
     for (int it = 0; it < tiles; ++it) {
       const int s = it % Stages, round = it / Stages;
@@ -273,15 +321,15 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
         load_boxes<Boxes, kBN>(smem_addr(sm.q[s]), &maps.q, full, t.base + q0, h, t.ev);
         load_boxes<Boxes, kBN>(smem_addr(sm.g[s]), &maps.g, full, t.base + q0, h, t.ev);
       }
-      const int64_t st = stat_at(p, t, p.heads, h, q0);
+      const float* st = stats + stat_at(p, t, p.heads, h, q0);
 #pragma unroll
       for (int r = lane; r < kBN; r += 32) {
         const bool live = q0 + r < t.len;
-        sm.lse2n[s][r] = live ? a.lse[st + r] * -kLog2e : 0.f;
-        sm.deltan[s][r] = live ? -a.delta[st + r] : 0.f;
+        const float* src = live ? st + r : stats;
+        copy4(smem_addr(&sm.lse2n[s][r]), src, live);
+        copy4(smem_addr(&sm.deltan[s][r]), src + (live ? p.total_rows * p.heads : 0), live);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(full);
+      async_arrive(full);
       q0 += kBN;
       if (q0 >= t.len) {
         q0 = first;
@@ -292,117 +340,154 @@ __global__ void __launch_bounds__(col_threads(Groups), Groups == 1 ? 2 : 1)
     const uint32_t leader = elect_one();
     const int n = uniform(tiles), each = uniform(per_head), rows = uniform(t.len - first);
     const int dim = uniform(D);
-    const uint32_t mem = uniform(tmem), v_mem = mem + Groups * 128, k_mem = v_mem + kAcc;
+    const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, v_mem = p_mem + kBN,
+                   k_mem = v_mem + kAcc;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
     auto rows_of = [&](int it) { return min(kBN, rows - it % each * kBN); };
-    // S^T and dP^T of a tile into its group's accumulators. The MMAs run in
-    // order, so those that read the tile before from there are done.
+    // S^T over P^T and dP^T over dS^T: MMAs complete in order, so the products
+    // that read those are done.
     auto logits = [&](int it) {
-      const int s = it % Stages, w = it % Groups, up = (rows_of(it) + 15) & ~15;
-      if (!mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1)) return false;
-      product<T, Boxes, kBM, kBN>(mem + w * 128, smem_addr(sm.k), smem_addr(sm.q[s]), dim, up,
-                                  p.scale < 0.f, leader);
-      product<T, Boxes, kBM, kBN>(mem + w * 128 + 64, smem_addr(sm.v), smem_addr(sm.g[s]), dim,
-                                  up, false, leader);
-      tc_commit(smem_addr(&sm.s_full[w]), leader);
+      if (!mbar_wait(smem_addr(&sm.full[it % Stages]), (it / Stages) & 1)) return false;
+      product<T, Boxes, kBM, kBN>(s_mem, smem_addr(sm.k), smem_addr(sm.q[it % Stages]), dim,
+                                  (rows_of(it) + 15) & ~15, p.scale < 0.f, leader);
+      tc_commit(smem_addr(&sm.s_full), leader);
       return true;
     };
-    ok = mbar_wait(smem_addr(&sm.own_full), 0);
-    for (int it = 0; it < Groups && it < n && ok; ++it) ok = logits(it);
+    auto weights = [&](int it) {
+      product<T, Boxes, kBM, kBN>(p_mem, smem_addr(sm.v), smem_addr(sm.g[it % Stages]), dim,
+                                  (rows_of(it) + 15) & ~15, false, leader);
+      tc_commit(smem_addr(&sm.dp_full), leader);
+    };
+    ok = mbar_wait(smem_addr(&sm.own_full), 0) && logits(0);
+    if (ok) weights(0);
     for (int it = 0; it < n && ok; ++it) {
-      const int s = it % Stages, w = it % Groups, q_rows = rows_of(it);
-      ok = mbar_wait(smem_addr(&sm.ready[w]), (it / Groups) & 1);
+      const int s = it % Stages;
+      ok = mbar_wait(smem_addr(&sm.p_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
-      accumulate<kBN>(v_mem, mem + w * 128, smem_addr(sm.g[s]), q_rows, acc_instr, it > 0, leader);
-      accumulate<kBN>(k_mem, mem + w * 128 + 64, smem_addr(sm.q[s]), q_rows, acc_instr, it > 0,
-                      leader);
+      accumulate<kBN>(v_mem, s_mem, smem_addr(sm.g[s]), rows_of(it), acc_instr, it > 0, leader);
+      if (it + 1 < n) ok = logits(it + 1);
+      ok = ok && mbar_wait(smem_addr(&sm.ds_ready), it & 1);
+      if (!ok) break;
+      tc_fence_after();
+      accumulate<kBN>(k_mem, p_mem, smem_addr(sm.q[s]), rows_of(it), acc_instr, it > 0, leader);
       tc_commit(smem_addr(&sm.empty[s]), leader);
-      if (it + Groups < n) ok = logits(it + Groups);
+      if (it + 1 < n) weights(it + 1);
     }
     if (ok) tc_commit(smem_addr(&sm.done), leader);
   } else {
-    const int w = warp / 4;
+    const int w = warp / 4;  // query columns [64 w, +64) of a tile
     const uint32_t quad = (uint32_t)(warp % 4 * 32) << 16;
-    const uint32_t tS = tmem + w * 128 + quad, tP = tS + 64;
+    const uint32_t tS = tmem + quad + w * 64, tP = tS + kBN;
     const int j = t.i0 + warp % 4 * 32 + lane;
     const float c2 = fabsf(p.scale) * kLog2e;
     const pair_t scale2 = pair(c2, c2);
-    for (int it = w; it < tiles; it += Groups) {
+    for (int it = 0; it < tiles; ++it) {
       const int s = it % Stages;
-      const int q0 = first + it % per_head * kBN, nq = min(kBN, t.len - q0);
-      const bool edge = nq < kBN || (p.causal && q0 < t.i0 + kBM - 1);
-      const int lo = p.causal ? j - q0 : 0;  // query columns lo <= c < nq see key j
+      const int q0 = first + it % per_head * kBN, all = min(kBN, t.len - q0);
+      const int qw = q0 + w * 64, nq = t.len - qw;  // this group's columns
+      const bool edge = nq < 64 || (p.causal && qw < t.i0 + kBM - 1);
+      const int lo = p.causal ? j - qw : 0;  // columns lo <= c < nq see key j
+      const float* ls = &sm.lse2n[s][w * 64];
+      const float* de = &sm.deltan[s][w * 64];
       ok = mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1) &&
-           mbar_wait(smem_addr(&sm.s_full[w]), (it / Groups) & 1);
+           mbar_wait(smem_addr(&sm.s_full), it & 1);
       if (!ok) break;
       tc_fence_after();
+      float x[2][32];
 #pragma unroll
-      for (int c = 0; c < kBN / 32; ++c) {
+      for (int c = 0; c < 2; ++c)
+        if (c * 32 < nq) tmem_ld32(x[c], tS + c * 32);
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
         if (c * 32 >= nq) continue;
-        float x[32], dp[32];
-        tmem_ld32(x, tS + c * 32);
-        tmem_ld32(dp, tP + c * 32);
-        tmem_wait_ld();
-        pin(x);
-        pin(dp);
+        pin(x[c]);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          const ulonglong2 ls = *(const ulonglong2*)&sm.lse2n[s][c * 32 + e];
-          const ulonglong2 de = *(const ulonglong2*)&sm.deltan[s][c * 32 + e];
+          const ulonglong2 l4 = *(const ulonglong2*)(ls + c * 32 + e);
 #pragma unroll
           for (int f = 0; f < 4; f += 2) {
-            float2 y = split(fma2(pair(x[e + f], x[e + f + 1]), scale2, f ? ls.y : ls.x));
-            y.x = ex2(y.x);
-            y.y = ex2(y.y);
-            const float2 ds = split(mul2(
-                pair(y.x, y.y), add2(pair(dp[e + f], dp[e + f + 1]), f ? de.y : de.x)));
-            x[e + f] = y.x;
-            x[e + f + 1] = y.y;
-            dp[e + f] = ds.x;
-            dp[e + f + 1] = ds.y;
+            const float2 y =
+                split(fma2(pair(x[c][e + f], x[c][e + f + 1]), scale2, f ? l4.y : l4.x));
+            x[c][e + f] = ex2(y.x);
+            x[c][e + f + 1] = ex2(y.y);
           }
         }
         if (edge) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const bool seen = c * 32 + e >= lo && c * 32 + e < nq;
-            x[e] = seen ? x[e] : 0.f;
-            dp[e] = seen ? dp[e] : 0.f;
+            const int col = c * 32 + e;
+            x[c][e] = col >= lo && col < nq ? x[c][e] : 0.f;
           }
         }
-        uint32_t wp[16], wd[16];
+        uint32_t y[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          wp[e] = Elem<T>::pack(x[2 * e], x[2 * e + 1]);
-          wd[e] = Elem<T>::pack(dp[2 * e], dp[2 * e + 1]);
-        }
-        tmem_st16(tS + c * 16, wp);
-        tmem_st16(tP + c * 16, wd);
+        for (int e = 0; e < 16; ++e) y[e] = Elem<T>::pack(x[c][2 * e], x[c][2 * e + 1]);
+        tmem_st16(tS + c * 16, y);
       }
-      if (nq & 15) {
-        zero_tile_rows<Boxes, kBN>(sm.q[s], nq, (nq + 15) & ~15, threadIdx.x & 127, 128);
-        zero_tile_rows<Boxes, kBN>(sm.g[s], nq, (nq + 15) & ~15, threadIdx.x & 127, 128);
+      if (all & 15) {
+        // Rows up to the next multiple of 16 have P = dS = 0, and must not meet
+        // another event's NaN. (A dP^T still reading dO there is masked.)
+        zero_tile_rows<Boxes, kBN>(sm.q[s], all, (all + 15) & ~15, threadIdx.x, W * 128);
+        zero_tile_rows<Boxes, kBN>(sm.g[s], all, (all + 15) & ~15, threadIdx.x, W * 128);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&sm.ready[w]));
+      if (lane == 0) mbar_arrive(smem_addr(&sm.p_ready));
+      ok = mbar_wait(smem_addr(&sm.dp_full), it & 1);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (c * 32 >= nq) continue;
+        float dp[32];
+        tmem_ld32(dp, tP + c * 32);
+        tmem_wait_ld();
+        pin(dp);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const ulonglong2 d4 = *(const ulonglong2*)(de + c * 32 + e);
+#pragma unroll
+          for (int f = 0; f < 4; f += 2) {
+            const float2 y = split(mul2(pair(x[c][e + f], x[c][e + f + 1]),
+                                        add2(pair(dp[e + f], dp[e + f + 1]), f ? d4.y : d4.x)));
+            dp[e + f] = y.x;
+            dp[e + f + 1] = y.y;
+          }
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int col = c * 32 + e;
+            dp[e] = col >= lo && col < nq ? dp[e] : 0.f;
+          }
+        }
+        uint32_t y[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = Elem<T>::pack(dp[2 * e], dp[2 * e + 1]);
+        tmem_st16(tP + c * 16, y);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&sm.ds_ready));
     }
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
-    // The groups share the epilogue: one of two stores dV, the other dK.
+    // One of two groups stores dV, the other dK.
     const bool live = j < t.len;
+    const uint32_t tV = tmem + quad + 2 * kBN, tK = tV + kAcc;
     if (w == 0)
-      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, tV + quad, D, ok ? 1.f : NAN);
-    if (w == Groups - 1)
-      store_row<T>(live ? row_ptr<T>(a.dk, t, kh, j) : nullptr, tK + quad, D,
-                   ok ? p.scale : NAN);
+      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, tV, D, ok ? 1.f : NAN);
+    if (w == W - 1)
+      store_row<T>(live ? row_ptr<T>(a.dk, t, kh, j) : nullptr, tK, D, ok ? p.scale : NAN);
     tc_fence_before();
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == kTma) tmem_free<kCols>(tmem);
+  if (warp == kMma) tmem_free<kCols>(tmem);
 }
 
 template <typename K>
@@ -412,41 +497,40 @@ int prepare(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return FST_OK;
 }
 
-template <typename T, int Boxes, int RowStages, int ColStages, int Groups>
+template <typename T, int Boxes, int W, int RowStages, int ColStages>
 int launch(const FstGroupedBackwardArgs& a, cudaStream_t st) {
   const FstGroupedProblem& p = a.prob;
   static std::atomic<uint64_t> row_done{0}, col_done{0};
-  const auto rows_k = dq_kernel<T, Boxes, RowStages>;
-  const auto cols_k = dkv_kernel<T, Boxes, ColStages, Groups>;
-  const int row_bytes = (int)sizeof(RowSmem<Boxes, RowStages>) + 1024;
-  const int col_bytes = (int)sizeof(ColSmem<Boxes, ColStages, Groups>) + 1024;
+  const auto rows_k = dq_kernel<T, Boxes, W, RowStages>;
+  const auto cols_k = dkv_kernel<T, Boxes, W, ColStages>;
+  const int row_bytes = (int)sizeof(RowSmem<Boxes, W, RowStages>) + 1024;
+  const int col_bytes = (int)sizeof(ColSmem<Boxes, W, ColStages>) + 1024;
   int rc = prepare(rows_k, row_bytes, row_done);
   if (!rc) rc = prepare(cols_k, col_bytes, col_done);
   const int64_t rows = p.packed ? p.total_rows : p.max_len, events = p.packed ? 1 : p.batch;
-  const int D = p.head_dim;
-  TileMaps r, c;  // 128 own rows, 64 of the other side
+  const int D = p.head_dim, other = W * 64;
+  TileMaps r, c;  // 128 own rows, 64 W of the other side
   if (!rc) rc = tc::make_rows_map(&r.q, a.q, D, rows, p.heads, events, kBM);
   if (!rc) rc = tc::make_rows_map(&r.g, a.dout, D, rows, p.heads, events, kBM);
-  if (!rc) rc = tc::make_rows_map(&r.k, a.k, D, rows, p.kv_heads, events, kBN);
-  if (!rc) rc = tc::make_rows_map(&r.v, a.v, D, rows, p.kv_heads, events, kBN);
-  if (!rc) rc = tc::make_rows_map(&c.q, a.q, D, rows, p.heads, events, kBN);
-  if (!rc) rc = tc::make_rows_map(&c.g, a.dout, D, rows, p.heads, events, kBN);
-  if (!rc) rc = tc::make_rows_map(&c.k, a.k, D, rows, p.kv_heads, events, kBM);
-  if (!rc) rc = tc::make_rows_map(&c.v, a.v, D, rows, p.kv_heads, events, kBM);
+  if (!rc) rc = tc::make_rows_map(&r.k, a.k, D, rows, p.kv_heads, events, other);
+  if (!rc) rc = tc::make_rows_map(&r.v, a.v, D, rows, p.kv_heads, events, other);
+  if (!rc && W == 2) c = r;  // the same boxes
+  if (!rc && W == 1) rc = tc::make_rows_map(&c.q, a.q, D, rows, p.heads, events, other);
+  if (!rc && W == 1) rc = tc::make_rows_map(&c.g, a.dout, D, rows, p.heads, events, other);
+  if (!rc && W == 1) rc = tc::make_rows_map(&c.k, a.k, D, rows, p.kv_heads, events, kBM);
+  if (!rc && W == 1) rc = tc::make_rows_map(&c.v, a.v, D, rows, p.kv_heads, events, kBM);
   if (rc) return rc;
   const int blocks = (int)list_blocks(p, kBM);
-  rows_k<<<(unsigned)(blocks * p.heads), kRowThreads, row_bytes, st>>>(r, a, blocks);
-  cols_k<<<(unsigned)(blocks * p.kv_heads), col_threads(Groups), col_bytes, st>>>(c, a, blocks);
+  rows_k<<<(unsigned)(blocks * p.heads), threads_of(W), row_bytes, st>>>(r, a, blocks, a.stats);
+  cols_k<<<(unsigned)(blocks * p.kv_heads), threads_of(W), col_bytes, st>>>(c, a, blocks, a.stats);
   count_launch(2);
   return FST_OK;
 }
 
 template <typename T>
 int launch_t(const FstGroupedBackwardArgs& a, cudaStream_t st) {
-  // Two blocks an SM where dK and dV of 64 columns leave tensor memory for
-  // them; else one block with two groups.
-  if (a.prob.head_dim <= 64) return launch<T, 1, 3, 4, 1>(a, st);
-  return launch<T, 2, 1, 4, 2>(a, st);
+  if (a.prob.head_dim <= 64) return launch<T, 1, 1, 3, 4>(a, st);
+  return launch<T, 2, 2, 2, 2>(a, st);
 }
 
 }  // namespace

@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(FstGroupedBackwardArgs a) 
     delta[r] = half_warp_sum(sum);
     const int64_t at = stat_at(p, t, p.heads, h, i);
     lse2[r] = i < t.len ? a.lse[at] * kLog2e : 0.f;
-    if (tx == 0 && i < t.len) a.delta[at] = delta[r];
+    if (tx == 0 && i < t.len) a.stats[at] = delta[r];
   }
   const int end = p.causal ? min(t.len, t.i0 + kB) : t.len;
   for (int j0 = 0; j0 < end; j0 += kB) {
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(FstGroupedBackwardArgs a)
         const bool live = q0 + (int)threadIdx.x < t.len;
         const int64_t at = stat_at(p, t, p.heads, h, q0 + threadIdx.x);
         lse2[threadIdx.x] = live ? a.lse[at] * kLog2e : 0.f;
-        delta[threadIdx.x] = live ? a.delta[at] : 0.f;
+        delta[threadIdx.x] = live ? a.stats[at] : 0.f;
       }
       __syncthreads();
       float s[4][4], dp[4][4];  // [key row][query column]

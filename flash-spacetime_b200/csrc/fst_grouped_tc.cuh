@@ -231,6 +231,17 @@ __device__ __forceinline__ void load_boxes(uint32_t dst, const CUtensorMap* map,
   for (int b = 0; b < Boxes; ++b) load_box(dst + b * Rows * 128, map, bar, b * 64, row, h, ev);
 }
 
+// Four bytes from global to shared memory, or zero; lands on the barrier that
+// async_arrive names (one arrival of each thread).
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(live ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // Zeros rows [first, last) of a tile (whole rows, so the swizzle does not
 // matter), by `n` threads of index t; made visible to the tensor cores.
 template <int Boxes, int Rows>
@@ -255,14 +266,16 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t A, uint32_t B, int 
              b + ((c / 4) * BRows * 128 + (c % 4) * 32) / 16, instr, c > 0, leader);
 }
 // d[128][n] (+)= P X over `rows` rows (rounded up to 16) of X, a tile of BRows
-// rows; P 16-bit values in tensor memory.
+// rows; P 16-bit values in tensor memory, 64 rows of X in 32 columns, the
+// next 64 from 64 columns on.
 template <int BRows>
 __device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, int rows,
                                            uint32_t instr, bool add, uint32_t leader) {
   const uint64_t x = operand(X, BRows * 128);
 #pragma unroll
   for (int c = 0; c < BRows / 16; ++c)
-    if (c * 16 < rows) mma_ts(d, P + c * 8, x + c * 2048 / 16, instr, add || c > 0, leader);
+    if (c * 16 < rows)
+      mma_ts(d, P + c / 4 * 64 + c % 4 * 8, x + c * 2048 / 16, instr, add || c > 0, leader);
 }
 
 // The block's rows of no event: zeros, in 16-byte vectors, by n threads.

@@ -159,7 +159,7 @@ class FstGroupedBackwardArgs(ctypes.Structure):
         ("dk", FstRows),
         ("dv", FstRows),
         ("lse", ctypes.c_void_p),
-        ("delta", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
     ]
 
 

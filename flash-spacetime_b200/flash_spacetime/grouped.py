@@ -141,12 +141,12 @@ class _FlashGroupedAttention(torch.autograd.Function):
             dout = _in_place(grad_out)
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device)
                           for t in (q, k, v))
-            delta = torch.empty_like(lse)
+            stats = torch.empty(2 * lse.numel(), dtype=torch.float32, device=q.device)
             a = _lib.FstGroupedBackwardArgs()
             a.prob = _problem(q, k, layout, lens, ctx.scale, ctx.causal)
             a.q, a.k, a.v, a.out, a.dout = (_rows(t, layout) for t in (q, k, v, out, dout))
             a.dq, a.dk, a.dv = (_rows(t, layout) for t in (dq, dk, dv))
-            a.lse, a.delta = _ptr(lse), _ptr(delta)
+            a.lse, a.stats = _ptr(lse), _ptr(stats)
             rc = _timed_call("fst_grouped_backward", lib.fst_grouped_backward,
                              (ctypes.byref(a), _stream(q.device)), q.device)
         _lib.check(rc, "fst_grouped_backward")

@@ -269,10 +269,9 @@ typedef struct FstGroupedProblem {
   const int32_t* cu_seqlens; /* [B+1] device row offsets (packed)             */
 } FstGroupedProblem;
 
-/* Per-row statistics (lse, delta) are dense fp32 [B, H, L] (padded) or [H, T]
- * (packed). Rows of no event -- padding, or packed rows outside
- * [cu_seqlens[0], cu_seqlens[B]) -- are never read and are written 0 in out,
- * dq, dk and dv; their lse and delta are left as they were. */
+/* lse is dense fp32 [B, H, L] (padded) or [H, T] (packed). Rows of no event --
+ * padding, or packed rows outside [cu_seqlens[0], cu_seqlens[B]) -- are never
+ * read and are written 0 in out, dq, dk and dv; their lse is left as it was. */
 typedef struct FstGroupedForwardArgs {
   FstGroupedProblem prob;
   FstRows q;             /* H heads                                          */
@@ -293,7 +292,7 @@ typedef struct FstGroupedBackwardArgs {
   FstRows dk;
   FstRows dv;
   const float* lse;      /* from fst_grouped_forward                         */
-  float* delta;          /* output: D_i = dout_i . out_i                     */
+  float* stats;          /* device scratch: 2 * heads * total_rows floats    */
 } FstGroupedBackwardArgs;
 
 int fst_grouped_forward(const FstGroupedForwardArgs* args, void* stream);
