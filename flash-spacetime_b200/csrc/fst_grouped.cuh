@@ -61,18 +61,24 @@ __device__ __forceinline__ bool find_tile(const FstGroupedProblem& p, int id, bo
     t.lim = p.max_len;
   } else {
     // Largest entry whose position is <= id: 33-way search, one probe a lane.
+    // The rows at both ends of the range are kept, so that each step is the
+    // only trip to memory: one up to 31 events, two up to 1055.
     const int lane = threadIdx.x & 31;
-    int lo = -1, hi = p.batch + 1;
+    int lo = -1, hi = p.batch + 1, a = 0, b = (int)p.total_rows;
     while (hi - lo > 1) {
       const int step = (hi - lo + 32) / 33;
       const int e = lo + step * (lane + 1);
-      const bool at = e < hi && entry_row(p, e) / BM + e + 1 <= id;
-      const int n = __ffs(~__ballot_sync(0xffffffffu, at)) - 1;  // -1 + 1 .. 32
-      const int steps = n < 0 ? 32 : n;
-      lo += step * steps;
+      const int row = e < hi ? entry_row(p, e) : b;
+      const bool at = e < hi && row / BM + e + 1 <= id;
+      const int first = __ffs(~__ballot_sync(0xffffffffu, at)) - 1;
+      const int n = first < 0 ? 32 : first;  // probes at or below id
+      const int below = __shfl_sync(0xffffffffu, row, n > 0 ? n - 1 : 0);
+      const int above = __shfl_sync(0xffffffffu, row, n < 32 ? n : 31);
+      a = n > 0 ? below : a;
+      b = n < 32 ? above : b;
+      lo += step * n;
       hi = min(hi, lo + step);
     }
-    const int a = entry_row(p, lo), b = entry_row(p, lo + 1);
     t.ev = 0;
     t.base = a;
     t.lim = max(b - a, 0);

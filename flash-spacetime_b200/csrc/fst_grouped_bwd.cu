@@ -63,6 +63,24 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
   constexpr int kBN = W * 64, kCols = W * 256, kTma = W * 4, kMma = kTma + 1;
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (warp == kTma && lane == 0) {
+    mbar_init(smem_addr(&sm.own_full), 1);
+    for (int s = 0; s < Stages; ++s) {
+      mbar_init(smem_addr(&sm.full[s]), 1);
+      mbar_init(smem_addr(&sm.empty[s]), 1);
+    }
+    mbar_init(smem_addr(&sm.s_full), 1);
+    mbar_init(smem_addr(&sm.s_free), W * 4);
+    mbar_init(smem_addr(&sm.dp_full), 1);
+    mbar_init(smem_addr(&sm.ds_ready), W * 4);
+    mbar_init(smem_addr(&sm.done), 1);
+    mbar_init_fence();
+    prefetch_map(&maps.q);
+    prefetch_map(&maps.g);
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
+  __syncwarp();
   const BlockAt at = block_at(p, blocks);
   RowTile t;
   if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
@@ -80,17 +98,6 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     load_boxes<Boxes, kBN>(smem_addr(sm.v[s]), &maps.v, full, t.base + it * kBN, at.kh, t.ev);
   };
   if (warp == kTma && lane == 0) {
-    mbar_init(smem_addr(&sm.own_full), 1);
-    for (int s = 0; s < Stages; ++s) {
-      mbar_init(smem_addr(&sm.full[s]), 1);
-      mbar_init(smem_addr(&sm.empty[s]), 1);
-    }
-    mbar_init(smem_addr(&sm.s_full), 1);
-    mbar_init(smem_addr(&sm.s_free), W * 4);
-    mbar_init(smem_addr(&sm.dp_full), 1);
-    mbar_init(smem_addr(&sm.ds_ready), W * 4);
-    mbar_init(smem_addr(&sm.done), 1);
-    mbar_init_fence();
     // The first tiles set out before the others are ready for them.
     const uint32_t own = smem_addr(&sm.own_full);
     mbar_arrive_tx(own, 2 * Boxes * kBM * 128);
@@ -273,6 +280,24 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
   static_assert(kCols == 256 || kCols == 512, "tensor memory comes in powers of two");
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (warp == kTma && lane == 0) {
+    mbar_init(smem_addr(&sm.own_full), 1);
+    for (int s = 0; s < Stages; ++s) {
+      mbar_init(smem_addr(&sm.full[s]), 1 + 32);  // TMA, and each lane's copies
+      mbar_init(smem_addr(&sm.empty[s]), 1);
+    }
+    mbar_init(smem_addr(&sm.s_full), 1);
+    mbar_init(smem_addr(&sm.p_ready), W * 4);
+    mbar_init(smem_addr(&sm.dp_full), 1);
+    mbar_init(smem_addr(&sm.ds_ready), W * 4);
+    mbar_init(smem_addr(&sm.done), 1);
+    mbar_init_fence();
+    prefetch_map(&maps.q);
+    prefetch_map(&maps.g);
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
+  __syncwarp();
   const int kh = blockIdx.x / blocks, id = blockIdx.x - kh * blocks;
   const int group = p.heads / p.kv_heads;
   RowTile t;
@@ -286,17 +311,6 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
   const int tiles = per_head * group;
 
   if (warp == kTma && lane == 0) {
-    mbar_init(smem_addr(&sm.own_full), 1);
-    for (int s = 0; s < Stages; ++s) {
-      mbar_init(smem_addr(&sm.full[s]), 1 + 32);  // TMA, and each lane's copies
-      mbar_init(smem_addr(&sm.empty[s]), 1);
-    }
-    mbar_init(smem_addr(&sm.s_full), 1);
-    mbar_init(smem_addr(&sm.p_ready), W * 4);
-    mbar_init(smem_addr(&sm.dp_full), 1);
-    mbar_init(smem_addr(&sm.ds_ready), W * 4);
-    mbar_init(smem_addr(&sm.done), 1);
-    mbar_init_fence();
     const uint32_t own = smem_addr(&sm.own_full);
     mbar_arrive_tx(own, 2 * Boxes * kBM * 128);
     load_boxes<Boxes, kBM>(smem_addr(sm.k), &maps.k, own, t.base + t.i0, kh, t.ev);
@@ -338,41 +352,43 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     }
   } else if (warp == kMma) {
     const uint32_t leader = elect_one();
-    const int n = uniform(tiles), each = uniform(per_head), rows = uniform(t.len - first);
-    const int dim = uniform(D);
+    const int n = uniform(tiles), rows = uniform(t.len - first), dim = uniform(D);
     const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, v_mem = p_mem + kBN,
                    k_mem = v_mem + kAcc;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
-    auto rows_of = [&](int it) { return min(kBN, rows - it % each * kBN); };
     // S^T over P^T and dP^T over dS^T: MMAs complete in order, so the products
     // that read those are done.
-    auto logits = [&](int it) {
+    auto logits = [&](int it, int q_rows) {
       if (!mbar_wait(smem_addr(&sm.full[it % Stages]), (it / Stages) & 1)) return false;
       product<T, Boxes, kBM, kBN>(s_mem, smem_addr(sm.k), smem_addr(sm.q[it % Stages]), dim,
-                                  (rows_of(it) + 15) & ~15, p.scale < 0.f, leader);
+                                  (q_rows + 15) & ~15, p.scale < 0.f, leader);
       tc_commit(smem_addr(&sm.s_full), leader);
       return true;
     };
-    auto weights = [&](int it) {
+    auto weights = [&](int it, int q_rows) {
       product<T, Boxes, kBM, kBN>(p_mem, smem_addr(sm.v), smem_addr(sm.g[it % Stages]), dim,
-                                  (rows_of(it) + 15) & ~15, false, leader);
+                                  (q_rows + 15) & ~15, false, leader);
       tc_commit(smem_addr(&sm.dp_full), leader);
     };
-    ok = mbar_wait(smem_addr(&sm.own_full), 0) && logits(0);
-    if (ok) weights(0);
+    int done = 0, q_rows = min(kBN, rows);  // query rows of the head behind, of the tile
+    ok = mbar_wait(smem_addr(&sm.own_full), 0) && logits(0, q_rows);
+    if (ok) weights(0, q_rows);
     for (int it = 0; it < n && ok; ++it) {
       const int s = it % Stages;
+      done = done + kBN < rows ? done + kBN : 0;
+      const int next_rows = min(kBN, rows - done);
       ok = mbar_wait(smem_addr(&sm.p_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
-      accumulate<kBN>(v_mem, s_mem, smem_addr(sm.g[s]), rows_of(it), acc_instr, it > 0, leader);
-      if (it + 1 < n) ok = logits(it + 1);
+      accumulate<kBN>(v_mem, s_mem, smem_addr(sm.g[s]), q_rows, acc_instr, it > 0, leader);
+      if (it + 1 < n) ok = logits(it + 1, next_rows);
       ok = ok && mbar_wait(smem_addr(&sm.ds_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
-      accumulate<kBN>(k_mem, p_mem, smem_addr(sm.q[s]), rows_of(it), acc_instr, it > 0, leader);
+      accumulate<kBN>(k_mem, p_mem, smem_addr(sm.q[s]), q_rows, acc_instr, it > 0, leader);
       tc_commit(smem_addr(&sm.empty[s]), leader);
-      if (it + 1 < n) weights(it + 1);
+      if (it + 1 < n) weights(it + 1, next_rows);
+      q_rows = next_rows;
     }
     if (ok) tc_commit(smem_addr(&sm.done), leader);
   } else {
@@ -382,9 +398,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const int j = t.i0 + warp % 4 * 32 + lane;
     const float c2 = fabsf(p.scale) * kLog2e;
     const pair_t scale2 = pair(c2, c2);
-    for (int it = 0; it < tiles; ++it) {
-      const int s = it % Stages;
-      const int q0 = first + it % per_head * kBN, all = min(kBN, t.len - q0);
+    for (int it = 0, q0 = first; it < tiles; ++it, q0 = q0 + kBN < t.len ? q0 + kBN : first) {
+      const int s = it % Stages, all = min(kBN, t.len - q0);
       const int qw = q0 + w * 64, nq = t.len - qw;  // this group's columns
       const bool edge = nq < 64 || (p.causal && qw < t.i0 + kBM - 1);
       const int lo = p.causal ? j - qw : 0;  // columns lo <= c < nq see key j

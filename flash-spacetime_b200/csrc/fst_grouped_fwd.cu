@@ -52,6 +52,25 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kCols = 256;  // two S buffers (P over them) of kBN = 64, O from 128
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (warp == 4 && lane == 0) {
+    mbar_init(smem_addr(&sm.q_full), 1);
+    for (int s = 0; s < Stages; ++s) {
+      mbar_init(smem_addr(&sm.k_full[s]), 1);
+      mbar_init(smem_addr(&sm.k_empty[s]), 1);
+      mbar_init(smem_addr(&sm.v_full[s]), 1);
+      mbar_init(smem_addr(&sm.v_empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_addr(&sm.s_full[b]), 1);
+      mbar_init(smem_addr(&sm.p_ready[b]), 4);
+      mbar_init(smem_addr(&sm.pv_done[b]), 1);
+    }
+    mbar_init_fence();
+    prefetch_map(&maps.q);
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
+  __syncwarp();
   const BlockAt at = block_at(p, blocks);
   RowTile t;
   if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
@@ -67,19 +86,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     load_boxes<Boxes, kBN>(smem_addr(dst), map, bar, t.base + it * kBN, at.kh, t.ev);
   };
   if (warp == 4 && lane == 0) {
-    mbar_init(smem_addr(&sm.q_full), 1);
-    for (int s = 0; s < Stages; ++s) {
-      mbar_init(smem_addr(&sm.k_full[s]), 1);
-      mbar_init(smem_addr(&sm.k_empty[s]), 1);
-      mbar_init(smem_addr(&sm.v_full[s]), 1);
-      mbar_init(smem_addr(&sm.v_empty[s]), 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_addr(&sm.s_full[b]), 1);
-      mbar_init(smem_addr(&sm.p_ready[b]), 4);
-      mbar_init(smem_addr(&sm.pv_done[b]), 1);
-    }
-    mbar_init_fence();
     // The first tiles set out before the others are ready for them.
     mbar_arrive_tx(smem_addr(&sm.q_full), Boxes * kBM * 128);
     load_boxes<Boxes, kBM>(smem_addr(sm.q), &maps.q, smem_addr(&sm.q_full), t.base + t.i0, at.h,

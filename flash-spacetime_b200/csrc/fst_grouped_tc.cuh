@@ -213,6 +213,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // ---- TMA --------------------------------------------------------------------
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // Box of 64 channels from `c` (a multiple of 64: 128 bytes), rows from `row`
 // of head `h` of event `ev`. Rows and channels past the tensor read as zeros.
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c,
