@@ -115,55 +115,67 @@ __device__ __forceinline__ bool position_of(const FstRotaryArgs& p, int64_t row,
   return true;
 }
 
+// Quotients of a block's item numbers: n / d = umulhi(n, ceil(2^32 / d)) while
+// n d < 2^32, which the host makes sure of (a 32-bit division would cost more
+// instructions than the rotation).
+struct Split {
+  int rows_per_block, heads, slots;
+  uint32_t by_heads, by_slots;  // 0: the divisor is 1
+};
+__device__ __forceinline__ int quotient(int n, uint32_t by) {
+  return by ? (int)__umulhi((uint32_t)n, by) : n;
+}
+
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(FstRotaryArgs p, int rows_per_block,
-                                                          int slots) {
+__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(FstRotaryArgs p, Split sp) {
   __shared__ float2 cs[kMaxTable];
   __shared__ double pos[kMaxRows];
   __shared__ int live[kMaxRows];
-  __shared__ int64_t offs[kMaxRows][4];  // element offset of the row: q, q_out, k, k_out
-  const int64_t row0 = (int64_t)blockIdx.x * rows_per_block;
-  const int rows = (int)min((int64_t)rows_per_block, p.total_rows - row0);
-  const int heads = p.heads + (p.k.data ? p.kv_heads : 0);
-  if (threadIdx.x < rows) {
-    const int64_t row = row0 + threadIdx.x;
-    const int64_t ev = p.packed ? 0 : row / p.max_len;
-    const int64_t i = p.packed ? row : row - ev * p.max_len;
-    int64_t at = 0;
-    live[threadIdx.x] = position_of(p, row, i, at);
-    pos[threadIdx.x] = (double)at;
-    offs[threadIdx.x][0] = ev * p.q.event_stride + i * p.q.row_stride;
-    offs[threadIdx.x][1] = ev * p.q_out.event_stride + i * p.q_out.row_stride;
-    offs[threadIdx.x][2] = ev * p.k.event_stride + i * p.k.row_stride;
-    offs[threadIdx.x][3] = ev * p.k_out.event_stride + i * p.k_out.row_stride;
-  }
-  __syncthreads();
+  const int64_t row0 = (int64_t)blockIdx.x * sp.rows_per_block;
+  const int rows = (int)min((int64_t)sp.rows_per_block, p.total_rows - row0);
+  // Padded: event and row of the block's first row.
+  const int64_t ev0 = p.packed ? 0 : row0 / p.max_len;
+  const int64_t i0 = p.packed ? row0 : row0 - ev0 * p.max_len;
   using W = Vec<T, V>;
-  const int items = rows * heads * slots;  // host: below 2^31
+  const int items = rows * sp.heads * sp.slots;  // host: below 2^31
   for (int base = 0; base < items; base += kThreads * kItems) {
     W a[kItems], b[kItems];
     T* dst[kItems];
-    Slot slot[kItems];
-    int row[kItems];
+    int where[kItems];  // row of the block and slot of the head
 #pragma unroll
     for (int n = 0; n < kItems; ++n) {
       const int item = base + n * kThreads + threadIdx.x;
       dst[n] = nullptr;
       if (item >= items) continue;
-      const int s = item % slots, rh = item / slots;
-      const int h = rh % heads, r = rh / heads;
-      row[n] = r;
-      slot[n] = slot_at<V>(p, s);
+      const int rh = quotient(item, sp.by_slots), s = item - rh * sp.slots;
+      const int r = quotient(rh, sp.by_heads), h = rh - r * sp.heads;
+      where[n] = r << 16 | s;  // slots: at most 1024 / 2 + 1
+      const Slot t = slot_at<V>(p, s);
+      int64_t ev = ev0, i = i0 + r;
+      while (!p.packed && i >= p.max_len) {
+        i -= p.max_len;
+        ++ev;
+      }
       const bool is_k = h >= p.heads;
       const FstRows& in = is_k ? p.k : p.q;
       const FstRows& out = is_k ? p.k_out : p.q_out;
       const int hh = is_k ? h - p.heads : h;
-      const T* src = (const T*)in.data + offs[r][is_k ? 2 : 0] + hh * in.head_stride;
-      dst[n] = (T*)out.data + offs[r][is_k ? 3 : 1] + hh * out.head_stride;
-      a[n] = *(const W*)(src + slot[n].a);
-      if (slot[n].has_b) b[n] = *(const W*)(src + slot[n].b);
+      const T* src =
+          (const T*)in.data + ev * in.event_stride + i * in.row_stride + hh * in.head_stride;
+      dst[n] = (T*)out.data + ev * out.event_stride + i * out.row_stride + hh * out.head_stride;
+      a[n] = *(const W*)(src + t.a);
+      if (t.has_b) b[n] = *(const W*)(src + t.b);
     }
     if (base == 0) {
+      // The angles, while the loads are on their way.
+      if (threadIdx.x < rows) {
+        const int64_t at = row0 + threadIdx.x;
+        int64_t count = 0;
+        live[threadIdx.x] =
+            position_of(p, at, p.packed ? at : (i0 + threadIdx.x) % p.max_len, count);
+        pos[threadIdx.x] = (double)count;
+      }
+      __syncthreads();
       for (int e = threadIdx.x; e < rows * p.pairs; e += kThreads) {
         const int r = e / p.pairs;
         float sn = 0.f, c = 1.f;
@@ -180,9 +192,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(FstRotaryArgs p, int r
 #pragma unroll
     for (int n = 0; n < kItems; ++n) {
       if (!dst[n]) continue;
-      rotate<T, V>(p, slot[n], cs + row[n] * p.pairs, a[n], b[n]);
-      *(W*)(dst[n] + slot[n].a) = a[n];
-      if (slot[n].has_b) *(W*)(dst[n] + slot[n].b) = b[n];
+      const Slot t = slot_at<V>(p, where[n] & 0xffff);
+      rotate<T, V>(p, t, cs + (where[n] >> 16) * p.pairs, a[n], b[n]);
+      *(W*)(dst[n] + t.a) = a[n];
+      if (t.has_b) *(W*)(dst[n] + t.b) = b[n];
     }
   }
 }
@@ -204,22 +217,25 @@ int launch(const FstRotaryArgs& p, cudaStream_t st) {
   const int rot = p.interleaved ? (2 * p.pairs + 2 * w - 1) / (2 * w) : p.pairs / w;
   const int slots = p.interleaved ? (p.head_dim + 2 * w - 1) / (2 * w)
                                   : rot + (p.head_dim - 2 * p.pairs + 2 * w - 1) / (2 * w);
-  const int64_t row_items = (int64_t)(p.heads + (p.k.data ? p.kv_heads : 0)) * slots;
-  if (row_items * kMaxRows >= (1ll << 31))
-    return api_fail(FST_ERR_UNSUPPORTED, "rotary: %d heads of %d are too many", p.heads,
-                    p.head_dim);
+  const int heads = p.heads + (p.k.data ? p.kv_heads : 0);
+  const int64_t row_items = (int64_t)heads * slots;
   int64_t rows = kThreads * kItems / row_items;
   if (rows > kMaxRows) rows = kMaxRows;
   if (p.pairs > 0 && rows > kMaxTable / p.pairs) rows = kMaxTable / p.pairs;
   if (rows < 1) rows = 1;
+  if (row_items >= (1ll << 31) ||
+      rows * row_items * (heads > slots ? heads : slots) >= (1ll << 32))
+    return api_fail(FST_ERR_UNSUPPORTED, "rotary: %d heads of %d are too many", heads, p.head_dim);
   const int64_t blocks = (p.total_rows + rows - 1) / rows;
   if (blocks >= (1ll << 31))
     return api_fail(FST_ERR_UNSUPPORTED, "rotary: %lld rows are too many",
                     (long long)p.total_rows);
+  auto by = [](int d) { return d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u; };
+  const Split sp{(int)rows, heads, slots, by(heads), by(slots)};
   if (vec)
-    rotary_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(p, (int)rows, slots);
+    rotary_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(p, sp);
   else
-    rotary_kernel<T, 1><<<(unsigned)blocks, kThreads, 0, st>>>(p, (int)rows, slots);
+    rotary_kernel<T, 1><<<(unsigned)blocks, kThreads, 0, st>>>(p, sp);
   count_launch();
   return FST_OK;
 }

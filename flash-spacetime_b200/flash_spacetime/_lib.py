@@ -227,13 +227,10 @@ def load() -> ctypes.CDLL:
         lib.fst_upload_rows.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                         ctypes.c_int64, ctypes.c_void_p]
-        lib.fst_grouped_forward.restype = ctypes.c_int
-        lib.fst_grouped_forward.argtypes = [ctypes.POINTER(FstGroupedForwardArgs), ctypes.c_void_p]
-        lib.fst_grouped_backward.restype = ctypes.c_int
-        lib.fst_grouped_backward.argtypes = [ctypes.POINTER(FstGroupedBackwardArgs),
-                                             ctypes.c_void_p]
-        lib.fst_rotary.restype = ctypes.c_int
-        lib.fst_rotary.argtypes = [ctypes.POINTER(FstRotaryArgs), ctypes.c_void_p]
+        # Argument structs of these are passed as packed bytes (grouped.py) or byref.
+        for entry in (lib.fst_grouped_forward, lib.fst_grouped_backward, lib.fst_rotary):
+            entry.restype = ctypes.c_int
+            entry.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         lib.fst_kernel_launches.restype = ctypes.c_int64
         lib.fst_last_error.restype = ctypes.c_int
         lib.fst_last_error.argtypes = [ctypes.c_char_p, ctypes.c_size_t]

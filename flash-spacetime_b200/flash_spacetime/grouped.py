@@ -19,15 +19,26 @@ Conventions:
   a head are adjacent: slices of a fused projection need no copy.
 """
 
-import ctypes
-from typing import Any, Optional, Tuple
+import struct
+from typing import Any, Callable, Optional, Tuple
 
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPES, _padded_lengths, _ptr, _stream, _timed_call
+from .ops import _DTYPES, _padded_lengths, _timed_call
+
+# The argument structs of the C ABI, packed in one go: filling ctypes
+# structures field by field would take longer than a small call's kernels.
+# FstRows is (data, event, head, row stride).
+_PROBLEM = "8iqfi2Q"
+_ROWS = "Q3q"
+_FORWARD = struct.Struct("@" + _PROBLEM + 4 * _ROWS + "Q")
+_BACKWARD = struct.Struct("@" + _PROBLEM + 8 * _ROWS + "2Q")
+_CONTIGUOUS = torch.contiguous_format
+
+Sizes = Tuple[int, int, int, int]
 
 
 def _in_place(t: Tensor) -> Tensor:
@@ -37,28 +48,27 @@ def _in_place(t: Tensor) -> Tensor:
     For 16-bit tensors whose head is a whole number of 16-byte vectors, rows
     off the 16-byte grid are copied too: the tensor-core kernels need it.
     """
-    aligned = True
+    aligned = t.data_ptr() % 16 == 0
+    if aligned and t.is_contiguous():
+        return t
     if t.element_size() == 2 and t.shape[-1] % 8 == 0:
-        aligned = t.data_ptr() % 16 == 0 and all(
+        aligned = aligned and all(
             s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+    else:
+        aligned = True
     strided = all(s > 0 for s, n in zip(t.stride(), t.shape) if n > 1)
     if aligned and strided and (t.stride(-1) == 1 or t.shape[-1] == 1):
         return t
-    return t.clone(memory_format=torch.contiguous_format)
+    return t.clone(memory_format=_CONTIGUOUS)
 
 
-def _rows(t: Optional[Tensor], layout: str) -> _lib.FstRows:
-    r = _lib.FstRows()
-    if t is None:
-        return r
-    r.data = _ptr(t)
+def _rows(t: Tensor, layout: str) -> Tuple[int, int, int, int]:
+    s = t.stride()
     if layout == "packed":
-        r.row_stride, r.head_stride = t.stride(0), t.stride(1)
-    elif layout == "bhld":
-        r.event_stride, r.head_stride, r.row_stride = t.stride(0), t.stride(1), t.stride(2)
-    else:
-        r.event_stride, r.row_stride, r.head_stride = t.stride(0), t.stride(1), t.stride(2)
-    return r
+        return t.data_ptr(), 0, s[1], s[0]
+    if layout == "bhld":
+        return t.data_ptr(), s[0], s[1], s[2]
+    return t.data_ptr(), s[0], s[2], s[1]
 
 
 def _integers(t: Tensor, what: str) -> Tensor:
@@ -67,20 +77,21 @@ def _integers(t: Tensor, what: str) -> Tensor:
     return t
 
 
-def _shape(t: Tensor, layout: str, what: str) -> Tuple[int, int, int, int]:
+def _shape(t: Tensor, layout: str, what: str) -> Sizes:
     """(events, rows per event or in all, heads, Dh) of a tensor."""
+    shape = t.shape
     if layout == "packed":
-        if t.dim() != 3:
-            raise ValueError(f"varlen {what} must be [T, H, D], got {tuple(t.shape)}")
-        return 0, t.shape[0], t.shape[1], t.shape[2]
+        if len(shape) != 3:
+            raise ValueError(f"varlen {what} must be [T, H, D], got {tuple(shape)}")
+        return 0, shape[0], shape[1], shape[2]
     if layout not in ("bhld", "blhd"):
         raise ValueError(f"layout must be 'bhld' or 'blhd', got {layout!r}")
-    if t.dim() != 4:
+    if len(shape) != 4:
         raise ValueError(f"{what} must be [B, H, L, D] (or [B, L, H, D] with layout='blhd'), "
-                         f"got {tuple(t.shape)}")
+                         f"got {tuple(shape)}")
     if layout == "blhd":
-        return t.shape[0], t.shape[1], t.shape[2], t.shape[3]
-    return t.shape[0], t.shape[2], t.shape[1], t.shape[3]
+        return shape[0], shape[1], shape[2], shape[3]
+    return shape[0], shape[2], shape[1], shape[3]
 
 
 def _check_tensor(t: Tensor, q: Tensor, what: str) -> None:
@@ -92,43 +103,54 @@ def _check_tensor(t: Tensor, q: Tensor, what: str) -> None:
         raise ValueError("q, k and v must have the same dtype")
 
 
-def _problem(q: Tensor, k: Tensor, layout: str, lens: Tensor, scale: float,
-             causal: bool) -> _lib.FstGroupedProblem:
+def _on_device(index: int, run: Callable[[int], Any]) -> Any:
+    """``run(stream)`` with the device current and its current stream."""
+    if torch.cuda.current_device() == index:
+        return run(torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return run(torch._C._cuda_getCurrentRawStream(index))
+
+
+def _call(name: str, args: bytes, device: torch.device) -> None:
+    entry = getattr(_lib.load(), name)
+    rc = _on_device(device.index,
+                    lambda stream: _timed_call(name, entry, (args, stream), device))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _problem(q: Tensor, kv_heads: int, layout: str, lens: Tensor, scale: float,
+             causal: bool) -> Tuple[Any, ...]:
     events, rows, heads, dim = _shape(q, layout, "q")
-    p = _lib.FstGroupedProblem()
-    p.dtype = _DTYPES[q.dtype]
-    p.packed = int(layout == "packed")
-    p.heads, p.kv_heads = heads, _shape(k, layout, "k")[2]
-    p.head_dim, p.causal, p.scale = dim, int(causal), scale
-    if p.packed:
-        p.batch, p.total_rows, p.cu_seqlens = lens.numel() - 1, rows, _ptr(lens)
-    else:
-        p.batch, p.max_len, p.total_rows, p.seqlens = events, rows, events * rows, _ptr(lens)
-    return p
+    dtype = _DTYPES[q.dtype]
+    if layout == "packed":
+        return (dtype, 1, lens.shape[0] - 1, heads, kv_heads, 0, dim, causal, rows, scale, 0,
+                0, lens.data_ptr())
+    return (dtype, 0, events, heads, kv_heads, rows, dim, causal, events * rows, scale, 0,
+            lens.data_ptr(), 0)
 
 
-def _lse_shape(q: Tensor, layout: str) -> Tuple[int, ...]:
+def _forward(q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str, scale: float,
+             causal: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """One ``fst_grouped_forward`` call: out, lse, and q, k, v as read."""
+    q, k, v = _in_place(q), _in_place(k), _in_place(v)
     events, rows, heads, _ = _shape(q, layout, "q")
-    return (heads, rows) if layout == "packed" else (events, heads, rows)
+    out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    shape = (heads, rows) if layout == "packed" else (events, heads, rows)
+    lse = torch.empty(shape, dtype=torch.float32, device=q.device)
+    args = _FORWARD.pack(
+        *_problem(q, _shape(k, layout, "k")[2], layout, lens, scale, causal), *_rows(q, layout),
+        *_rows(k, layout), *_rows(v, layout), *_rows(out, layout), lse.data_ptr())
+    _call("fst_grouped_forward", args, q.device)
+    return out, lse, q, k, v
 
 
 class _FlashGroupedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str,
                 scale: float, causal: bool) -> Tensor:  # type: ignore[override]
-        lib = _lib.load()
-        qc, kc, vc = _in_place(q), _in_place(k), _in_place(v)
-        with torch.cuda.device(q.device):
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            lse = torch.empty(_lse_shape(q, layout), dtype=torch.float32, device=q.device)
-            a = _lib.FstGroupedForwardArgs()
-            a.prob = _problem(qc, kc, layout, lens, scale, causal)
-            a.q, a.k, a.v, a.out = (_rows(t, layout) for t in (qc, kc, vc, out))
-            a.lse = _ptr(lse)
-            rc = _timed_call("fst_grouped_forward", lib.fst_grouped_forward,
-                             (ctypes.byref(a), _stream(q.device)), q.device)
-        _lib.check(rc, "fst_grouped_forward")
-        ctx.save_for_backward(qc, kc, vc, out, lse, lens)
+        out, lse, q, k, v = _forward(q, k, v, lens, layout, scale, causal)
+        ctx.save_for_backward(q, k, v, out, lse, lens)
         ctx.layout, ctx.scale, ctx.causal = layout, scale, causal
         return out
 
@@ -136,39 +158,46 @@ class _FlashGroupedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx: Any, grad_out: Tensor) -> Tuple[Optional[Tensor], ...]:  # type: ignore[override]
         q, k, v, out, lse, lens = ctx.saved_tensors
-        lib, layout = _lib.load(), ctx.layout
-        with torch.cuda.device(q.device):
-            dout = _in_place(grad_out)
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                          for t in (q, k, v))
-            stats = torch.empty(2 * lse.numel(), dtype=torch.float32, device=q.device)
-            a = _lib.FstGroupedBackwardArgs()
-            a.prob = _problem(q, k, layout, lens, ctx.scale, ctx.causal)
-            a.q, a.k, a.v, a.out, a.dout = (_rows(t, layout) for t in (q, k, v, out, dout))
-            a.dq, a.dk, a.dv = (_rows(t, layout) for t in (dq, dk, dv))
-            a.lse, a.stats = _ptr(lse), _ptr(stats)
-            rc = _timed_call("fst_grouped_backward", lib.fst_grouped_backward,
-                             (ctypes.byref(a), _stream(q.device)), q.device)
-        _lib.check(rc, "fst_grouped_backward")
+        layout = ctx.layout
+        dout = _in_place(grad_out)
+        dq, dk, dv = (torch.empty_like(t, memory_format=_CONTIGUOUS) for t in (q, k, v))
+        stats = torch.empty(2 * lse.numel(), dtype=torch.float32, device=q.device)
+        args = _BACKWARD.pack(
+            *_problem(q, _shape(k, layout, "k")[2], layout, lens, ctx.scale, ctx.causal),
+            *_rows(q, layout), *_rows(k, layout), *_rows(v, layout), *_rows(out, layout),
+            *_rows(dout, layout), *_rows(dq, layout), *_rows(dk, layout), *_rows(dv, layout),
+            lse.data_ptr(), stats.data_ptr())
+        _call("fst_grouped_backward", args, q.device)
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
                 None, None, None, None)
 
 
-def _check_heads(q: Tensor, k: Tensor, v: Tensor, layout: str) -> None:
+def _check_heads(q: Tensor, k: Tensor, v: Tensor, layout: str) -> Sizes:
     if q.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype}")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_tensor(t, q, name)
-    events, rows, heads, dim = _shape(q, layout, "q")
-    if _shape(k, layout, "k")[:2] != (events, rows) or k.shape[-1] != dim or v.shape != k.shape:
+    _check_tensor(q, q, "q")
+    _check_tensor(k, q, "k")
+    _check_tensor(v, q, "v")
+    sizes = events, rows, heads, dim = _shape(q, layout, "q")
+    k_events, k_rows, kv_heads, k_dim = _shape(k, layout, "k")
+    if (k_events, k_rows, k_dim) != (events, rows, dim) or v.shape != k.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have q's events, rows "
                          f"and Dh, q is {tuple(q.shape)}")
-    kv_heads = _shape(k, layout, "k")[2]
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"the heads of q ({heads}) must be a multiple of those of k ({kv_heads})")
     if not 1 <= dim <= 128:
         raise ValueError(f"Dh (={dim}) must be 1 to 128")
+    return sizes
+
+
+def _apply(q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str, scale: Optional[float],
+           causal: bool) -> Tensor:
+    args = (q, k, v, lens, layout, float(q.shape[-1]**-0.5 if scale is None else scale),
+            bool(causal))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _FlashGroupedAttention.apply(*args)
+    return _forward(*args)[0]
 
 
 def flash_grouped_attention(
@@ -198,8 +227,7 @@ def flash_grouped_attention(
     reach the rows of its event that do not see it. Padding rows may hold
     anything.
     """
-    _check_heads(q, k, v, layout)
-    events, rows, _, _ = _shape(q, layout, "q")
+    events, rows, _, _ = _check_heads(q, k, v, layout)
     if isinstance(seqlens, Tensor) and seqlens.dim() == 1:
         _integers(seqlens, "seqlens")
     lens, _ = _padded_lengths(seqlens, key_padding_mask, events, rows, q.device, validate_mask,
@@ -210,9 +238,7 @@ def flash_grouped_attention(
     lens = lens.to(device=q.device, dtype=torch.int32).contiguous()
     if lens.shape != (events,):
         raise ValueError(f"seqlens must be [B] = [{events}], got {tuple(lens.shape)}")
-    return _FlashGroupedAttention.apply(q, k, v, lens, layout,
-                                        float(q.shape[-1]**-0.5 if scale is None else scale),
-                                        bool(causal))
+    return _apply(q, k, v, lens, layout, scale, causal)
 
 
 def flash_grouped_attention_varlen(
@@ -239,6 +265,4 @@ def flash_grouped_attention_varlen(
     if cu.dtype == torch.int64:
         cu = cu.clamp(0, q.shape[0])
     cu = cu.to(device=q.device, dtype=torch.int32).contiguous()
-    return _FlashGroupedAttention.apply(q, k, v, cu, "packed",
-                                        float(q.shape[-1]**-0.5 if scale is None else scale),
-                                        bool(causal))
+    return _apply(q, k, v, cu, "packed", scale, causal)

@@ -7,16 +7,18 @@ gradient is the rotation by the opposite angle, so nothing of q and k is kept
 for the backward.
 """
 
-import ctypes
+import struct
 from typing import Any, Optional, Tuple
 
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .grouped import _check_tensor, _integers, _rows, _shape
-from .ops import _DTYPES, _ptr, _stream, _timed_call
+from .grouped import _CONTIGUOUS, _ROWS, _call, _check_tensor, _integers, _rows, _shape
+from .ops import _DTYPES
+
+_ROTARY = struct.Struct("@11ifq3Q" + 4 * _ROWS)
+_NO_ROWS = (0, 0, 0, 0)
 
 
 def _adjacent(t: Tensor) -> Tensor:
@@ -24,32 +26,28 @@ def _adjacent(t: Tensor) -> Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _rotate(q: Tensor, k: Optional[Tensor], layout: str, freqs: Tensor, cu: Optional[Tensor],
-            positions: Optional[Tensor], interleaved: bool, magnitude: float,
+def _rotate(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
+            positions: Optional[Tensor], layout: str, interleaved: bool, magnitude: float,
             inverse: bool) -> Tuple[Tensor, Optional[Tensor]]:
-    lib = _lib.load()
-    with torch.cuda.device(q.device):
-        q = _adjacent(q)
-        k = None if k is None else _adjacent(k)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        events, rows, heads, dim = _shape(q, layout, "q")
-        a = _lib.FstRotaryArgs()
-        a.dtype, a.packed, a.heads, a.head_dim = _DTYPES[q.dtype], int(layout == "packed"), heads, dim
-        a.kv_heads = 0 if k is None else _shape(k, layout, "k")[2]
-        if a.packed:
-            a.batch, a.total_rows = (0 if cu is None else cu.numel() - 1), rows
-        else:
-            a.batch, a.max_len, a.total_rows = events, rows, events * rows
-        a.pairs, a.interleaved, a.inverse = freqs.numel(), int(interleaved), int(inverse)
-        a.magnitude = magnitude
-        a.freqs, a.cu_seqlens, a.positions = _ptr(freqs), _ptr(cu), _ptr(positions)
-        a.positions_64 = int(positions is not None and positions.dtype == torch.int64)
-        a.q, a.k = _rows(q, layout), _rows(k, layout)
-        a.q_out, a.k_out = _rows(q_out, layout), _rows(k_out, layout)
-        rc = _timed_call("fst_rotary", lib.fst_rotary, (ctypes.byref(a), _stream(q.device)),
-                         q.device)
-    _lib.check(rc, "fst_rotary")
+    """One ``fst_rotary`` call."""
+    q = _adjacent(q)
+    q_out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    events, rows, heads, dim = _shape(q, layout, "q")
+    k_out, kv_heads, k_rows, k_out_rows = None, 0, _NO_ROWS, _NO_ROWS
+    if k is not None:
+        k = _adjacent(k)
+        k_out = torch.empty_like(k, memory_format=_CONTIGUOUS)
+        kv_heads, k_rows, k_out_rows = _shape(k, layout, "k")[2], _rows(k, layout), _rows(k_out, layout)
+    packed = layout == "packed"
+    batch = (0 if cu is None else cu.shape[0] - 1) if packed else events
+    args = _ROTARY.pack(
+        _DTYPES[q.dtype], packed, batch, heads, kv_heads, 0 if packed else rows, dim,
+        freqs.shape[0], interleaved, inverse,
+        positions is not None and positions.dtype == torch.int64, magnitude,
+        rows if packed else events * rows, freqs.data_ptr(), 0 if cu is None else cu.data_ptr(),
+        0 if positions is None else positions.data_ptr(), *_rows(q, layout), *k_rows,
+        *_rows(q_out, layout), *k_out_rows)
+    _call("fst_rotary", args, q.device)
     return q_out, k_out
 
 
@@ -61,7 +59,7 @@ class _FlashRotary(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(freqs, cu, positions)
         ctx.how = (layout, interleaved, magnitude)
-        return _rotate(q, k, layout, freqs, cu, positions, interleaved, magnitude, False)
+        return _rotate(q, k, freqs, cu, positions, layout, interleaved, magnitude, False)
 
     @staticmethod
     @once_differentiable
@@ -72,9 +70,9 @@ class _FlashRotary(torch.autograd.Function):
         gk = gk if ctx.needs_input_grad[1] else None
         dq = dk = None
         if gq is not None:
-            dq, dk = _rotate(gq, gk, layout, freqs, cu, positions, interleaved, magnitude, True)
+            dq, dk = _rotate(gq, gk, freqs, cu, positions, layout, interleaved, magnitude, True)
         elif gk is not None:
-            dk, _ = _rotate(gk, None, layout, freqs, cu, positions, interleaved, magnitude, True)
+            dk, _ = _rotate(gk, None, freqs, cu, positions, layout, interleaved, magnitude, True)
         return dq, dk, None, None, None, None, None, None
 
 
@@ -110,8 +108,10 @@ def _apply(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
         if positions.dtype not in (torch.int32, torch.int64):
             positions = positions.to(torch.int32)
         positions = positions.to(q.device).contiguous()
-    return _FlashRotary.apply(q, k, freqs, cu, positions, layout, bool(interleaved),
-                              float(magnitude))
+    args = (q, k, freqs, cu, positions, layout, bool(interleaved), float(magnitude))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _FlashRotary.apply(*args)
+    return _rotate(*args, False)
 
 
 def flash_rotary(
