@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     prefetch_map(&maps.v);
   }
   __syncwarp();
-  const BlockAt at = block_at(p, blocks);
+  const BlockAt at = block_at(p, blocks, blockIdx.x);
   RowTile t;
   if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
   const int D = p.head_dim;

@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "fst_grouped_tc.cuh"
 
@@ -38,7 +39,9 @@ struct FwdSmem {
   alignas(1024) char q[Boxes * kBM * 128];
   alignas(1024) char k[Stages][Boxes * kBN * 128];
   alignas(1024) char v[Stages][Boxes * kBN * 128];
-  uint64_t q_full, k_full[Stages], k_empty[Stages], v_full[Stages], v_empty[Stages];
+  Feed feed;
+  uint64_t q_full, q_empty, o_free;
+  uint64_t k_full[Stages], k_empty[Stages], v_full[Stages], v_empty[Stages];
   uint64_t s_full[2], p_ready[2], pv_done[2];  // of even and odd tiles
   uint32_t tmem;
 };
@@ -52,8 +55,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kCols = 256;  // two S buffers (P over them) of kBN = 64, O from 128
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int D = p.head_dim;
   if (warp == 4 && lane == 0) {
+    feed_init(sm.feed, 5);
     mbar_init(smem_addr(&sm.q_full), 1);
+    mbar_init(smem_addr(&sm.q_empty), 1);
+    mbar_init(smem_addr(&sm.o_free), 4);
     for (int s = 0; s < Stages; ++s) {
       mbar_init(smem_addr(&sm.k_full[s]), 1);
       mbar_init(smem_addr(&sm.k_empty[s]), 1);
@@ -70,179 +77,228 @@ __global__ void __launch_bounds__(kThreads, 2)
     prefetch_map(&maps.k);
     prefetch_map(&maps.v);
   }
-  __syncwarp();
-  const BlockAt at = block_at(p, blocks);
-  RowTile t;
-  if (!find_tile<kBM>(p, at.id, p.causal, t)) return;
-  const int D = p.head_dim;
-  zero_dead_rows<T, kBM>(a.out, t, at.h, D, kThreads);
-  if (t.i0 >= t.len) return;
-  const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
-  const int tiles = (end + kBN - 1) / kBN;
-
-  auto load = [&](int it, const CUtensorMap* map, char* dst, uint64_t* full) {
-    const uint32_t bar = smem_addr(full);
-    mbar_arrive_tx(bar, Boxes * kBN * 128);
-    load_boxes<Boxes, kBN>(smem_addr(dst), map, bar, t.base + it * kBN, at.kh, t.ev);
-  };
-  if (warp == 4 && lane == 0) {
-    // The first tiles set out before the others are ready for them.
-    mbar_arrive_tx(smem_addr(&sm.q_full), Boxes * kBM * 128);
-    load_boxes<Boxes, kBM>(smem_addr(sm.q), &maps.q, smem_addr(&sm.q_full), t.base + t.i0, at.h,
-                           t.ev);
-    for (int it = 0; it < Stages && it < tiles; ++it) {
-      load(it, &maps.k, sm.k[it], &sm.k_full[it]);
-      load(it, &maps.v, sm.v[it], &sm.v_full[it]);
-    }
-  }
   if (warp == 5) tmem_alloc<kCols>(smem_addr(&sm.tmem));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   const uint32_t tS = tmem, tO = tmem + 128;
+  // Two blocks that begin together would ask for the exponentials, and for the
+  // tensor cores, at the same time all along: the one in the upper half of
+  // tensor memory starts half a tile later.
+  if (tmem & 256) {
+    const uint32_t start = (uint32_t)clock();
+    while ((uint32_t)clock() - start < 600) {
+    }
+  }
 
+  // Barriers and buffers go by the tile's number n in the block's life; `live`
+  // counts its items that have tiles.
   bool ok = true;
   if (warp == 4) {
-    if (lane == 0) {
-      for (int it = Stages; it < tiles; ++it) {
-        const int s = it % Stages, last = (it / Stages - 1) & 1;
-        ok = mbar_wait(smem_addr(&sm.k_empty[s]), last);
-        if (!ok) break;
-        load(it, &maps.k, sm.k[s], &sm.k_full[s]);
-        ok = mbar_wait(smem_addr(&sm.v_empty[s]), last);
-        if (!ok) break;
-        load(it, &maps.v, sm.v[s], &sm.v_full[s]);
+    int c = 0, n = 0, live = 0, most = 0, index = blockIdx.x;
+    for (int round = 0; index >= 0 && ok; ++round) {
+      const BlockAt at = block_at(p, blocks, index);
+      Item item;
+      item.h = at.h;
+      item.kh = at.kh;
+      if (find_tile<kBM>(p, at.id, p.causal, item.t)) {
+        const RowTile& t = item.t;
+        const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
+        item.tiles = t.i0 < t.len ? (end + kBN - 1) / kBN : 0;
+        ok = feed_put(sm.feed, c++, item, most, lane);
+        if (item.tiles && ok) {
+          if (lane == 0) {
+            if (live) ok = wait_item(smem_addr(&sm.q_empty), (live - 1) & 1, most);
+            const uint32_t q_full = smem_addr(&sm.q_full);
+            if (ok) {
+              mbar_arrive_tx(q_full, Boxes * kBM * 128);
+              load_boxes<Boxes, kBM>(smem_addr(sm.q), &maps.q, q_full, t.base + t.i0, item.h,
+                                     t.ev);
+            }
+            for (int it = 0; it < item.tiles && ok; ++it) {
+              const int s = (n + it) % Stages, round_of = (n + it) / Stages;
+              auto load = [&](const CUtensorMap* map, char* dst, uint64_t* full, uint64_t* empty) {
+                if (round_of && !mbar_wait(smem_addr(empty), (round_of - 1) & 1)) return false;
+                const uint32_t bar = smem_addr(full);
+                mbar_arrive_tx(bar, Boxes * kBN * 128);
+                load_boxes<Boxes, kBN>(smem_addr(dst), map, bar, t.base + it * kBN, item.kh, t.ev);
+                return true;
+              };
+              ok = load(&maps.k, sm.k[s], &sm.k_full[s], &sm.k_empty[s]) &&
+                   load(&maps.v, sm.v[s], &sm.v_full[s], &sm.v_empty[s]);
+            }
+          }
+          n += item.tiles;
+          ++live;
+          most = max(most, item.tiles);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
       }
+      // Asked for only now, with the item's last loads under way, so that no
+      // block holds work that another has time for.
+      if (lane == 0) feed_ask(sm.feed);
+      __syncwarp();
+      index = feed_answer(sm.feed, round);
     }
+    Item last{};
+    last.tiles = -1;
+    feed_put(sm.feed, c, last, most, lane);
   } else if (warp == 5) {
     const uint32_t leader = elect_one();
-    const int n = uniform(tiles), last = uniform(end), dim = uniform(D);
+    const int dim = uniform(D);
     const uint32_t s_mem = uniform(tS), o_mem = s_mem + 128;
     const uint32_t o_instr = instruction<T>((dim + 15) & ~15, true, false);
-    auto keys = [&](int it) { return min(kBN, last - it * kBN); };
-    // S of a tile. Its buffer may be overwritten: MMAs complete in order,
-    // so the product that read P from it two tiles ago is done by then.
-    auto logits = [&](int it) {
-      const int s = it % Stages;
-      if (!mbar_wait(smem_addr(&sm.k_full[s]), (it / Stages) & 1)) return false;
-      product<T, Boxes, kBM, kBN>(s_mem + it % 2 * kBN, smem_addr(sm.q), smem_addr(sm.k[s]), dim,
-                                 (keys(it) + 15) & ~15, p.scale < 0.f, leader);
-      tc_commit(smem_addr(&sm.s_full[it % 2]), leader);
-      tc_commit(smem_addr(&sm.k_empty[s]), leader);
-      return true;
-    };
-    ok = mbar_wait(smem_addr(&sm.q_full), 0) && logits(0) && (n == 1 || logits(1));
-    for (int it = 0; it < n && ok; ++it) {
-      const int s = it % Stages;
-      ok = mbar_wait(smem_addr(&sm.v_full[s]), (it / Stages) & 1) &&
-           mbar_wait(smem_addr(&sm.p_ready[it % 2]), (it / 2) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      accumulate<kBN>(o_mem, s_mem + it % 2 * kBN, smem_addr(sm.v[s]), keys(it), o_instr, it > 0,
-                     leader);
-      tc_commit(smem_addr(&sm.pv_done[it % 2]), leader);
-      tc_commit(smem_addr(&sm.v_empty[s]), leader);
-      if (it + 2 < n) ok = logits(it + 2);
+    Item item;
+    for (int c = 0, n = 0, live = 0; ok && feed_take(sm.feed, c, item, lane); ++c) {
+      const int tiles = uniform(item.tiles);
+      if (!tiles) continue;
+      const int last =
+          uniform(p.causal ? min(item.t.len, item.t.i0 + kBM) : item.t.len);
+      auto keys = [&](int it) { return min(kBN, last - it * kBN); };
+      // S of a tile. Its buffer may be overwritten: MMAs complete in order,
+      // so the product that read P from it two tiles ago is done by then.
+      auto logits = [&](int it) {
+        const int g = n + it, s = g % Stages;
+        if (!mbar_wait(smem_addr(&sm.k_full[s]), (g / Stages) & 1)) return false;
+        product<T, Boxes, kBM, kBN>(s_mem + g % 2 * kBN, smem_addr(sm.q), smem_addr(sm.k[s]), dim,
+                                    (keys(it) + 15) & ~15, p.scale < 0.f, leader);
+        tc_commit(smem_addr(&sm.s_full[g % 2]), leader);
+        tc_commit(smem_addr(&sm.k_empty[s]), leader);
+        if (it + 1 == tiles) tc_commit(smem_addr(&sm.q_empty), leader);
+        return true;
+      };
+      ok = mbar_wait(smem_addr(&sm.q_full), live & 1) && logits(0) && (tiles == 1 || logits(1));
+      for (int it = 0; it < tiles && ok; ++it) {
+        const int g = n + it, s = g % Stages;
+        // The first product writes over O: the item before has read it.
+        if (it == 0 && live) ok = mbar_wait(smem_addr(&sm.o_free), (live - 1) & 1);
+        ok = ok && mbar_wait(smem_addr(&sm.v_full[s]), (g / Stages) & 1) &&
+             mbar_wait(smem_addr(&sm.p_ready[g % 2]), (g / 2) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        accumulate<kBN>(o_mem, s_mem + g % 2 * kBN, smem_addr(sm.v[s]), keys(it), o_instr, it > 0,
+                        leader);
+        tc_commit(smem_addr(&sm.pv_done[g % 2]), leader);
+        tc_commit(smem_addr(&sm.v_empty[s]), leader);
+        if (it + 2 < tiles) ok = logits(it + 2);
+      }
+      n += tiles;
+      ++live;
     }
   } else {
     const uint32_t quad = (uint32_t)(warp * 32) << 16;
-    const int i = t.i0 + warp * 32 + lane;
     // Above 0, so that a masked -inf stays -inf under a scale of 0.
     const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
-    float m = -INFINITY, l = 0.f;
-    for (int it = 0; it < tiles; ++it) {
-      const int j0 = it * kBN, nk = min(kBN, end - j0);
-      // Keys j0 <= j < j0 + lim are seen; `edge` when some row sees fewer
-      // than the tile's keys.
-      const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
-      const bool edge = j0 + kBN > t.len || (p.causal && j0 + kBN > t.i0 + 1);
-      const uint32_t tSt = tS + quad + it % 2 * kBN;
-      ok = mbar_wait(smem_addr(&sm.s_full[it % 2]), (it / 2) & 1);
-      // O += P V of two tiles ago: long done, but waited for, so that the
-      // wait on the last one below can only mean that one.
-      if (ok && it >= 2) ok = mbar_wait(smem_addr(&sm.pv_done[it % 2]), (it / 2 - 1) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      float s[kBN / 32][32];
+    const pair_t scale2 = pair(c2, c2);
+    Item item;
+    for (int c = 0, n = 0; ok && feed_take(sm.feed, c, item, lane); ++c) {
+      const RowTile& t = item.t;
+      zero_dead_rows<T, kBM>(a.out, t, item.h, D, 128);
+      if (!item.tiles) continue;
+      const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
+      const int i = t.i0 + warp * 32 + lane;
+      float m = -INFINITY, l = 0.f;
+      // One tile. `Whole`: every row of the block sees all its keys.
+      auto tile = [&](auto whole, int it) {
+        constexpr bool Whole = decltype(whole)::value;
+        const int j0 = it * kBN, nk = Whole ? kBN : min(kBN, end - j0);
+        const uint32_t tSt = tS + quad + n % 2 * kBN;
+        if (!mbar_wait(smem_addr(&sm.s_full[n % 2]), (n / 2) & 1)) return false;
+        tc_fence_after();
+        float s[2][32];
+        tmem_ld32(s[0], tSt);
+        if (Whole || nk > 32) tmem_ld32(s[1], tSt + 32);
+        tmem_wait_ld();
+        pin(s[0]);
+        pin(s[1]);
+        if (!Whole) {
+          // Keys below lim are seen; the warp's first row sees fewest.
+          const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0, fewest = uniform(lim);
 #pragma unroll
-      for (int c = 0; c < kBN / 32; ++c)
-        if (c * 32 < nk) tmem_ld32(s[c], tSt + c * 32);
-      tmem_wait_ld();
-      float mx = m;
+          for (int c = 0; c < 2; ++c) {
+            if (c * 32 + 32 <= fewest) continue;
 #pragma unroll
-      for (int c = 0; c < kBN / 32; ++c) {
-        if (c * 32 >= nk) continue;
-        pin(s[c]);
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e < lim ? s[c][e] : -INFINITY;
-        }
-        float part[4] = {mx, mx, mx, mx};
-#pragma unroll
-        for (int e = 0; e < 32; e += 8)
-#pragma unroll
-          for (int f = 0; f < 4; ++f)
-            part[f] = max3(part[f], s[c][e + 2 * f], s[c][e + 2 * f + 1]);
-        mx = max3(max3(part[0], part[1], part[2]), part[3], part[3]);
-      }
-      // First tile: O is written, not added to, so m may move freely.
-      if (it == 0) {
-        m = mx;
-      } else {
-        // (True for a NaN too, which then reaches O and l.)
-        const bool grow = !((mx - m) * c2 <= kGrow) && mx != m;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float keep = grow ? ex2((m - mx) * c2) : 1.f;
-          if (grow) {
-            m = mx;
-            l *= keep;
+            for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e < lim ? s[c][e] : -INFINITY;
           }
-          ok = mbar_wait(smem_addr(&sm.pv_done[(it - 1) % 2]), ((it - 1) / 2) & 1);
-          if (!ok) break;
-          tc_fence_after();
+        }
+        float part[8];
+#pragma unroll
+        for (int f = 0; f < 8; ++f) part[f] = max3(m, s[0][f], s[1][f]);
+#pragma unroll
+        for (int e = 8; e < 32; e += 8)
+#pragma unroll
+          for (int f = 0; f < 8; ++f) part[f] = max3(part[f], s[0][e + f], s[1][e + f]);
+        const float mx = max3(max3(part[0], part[1], part[2]), max3(part[3], part[4], part[5]),
+                              max3(part[6], part[7], part[7]));
+        // First tile: O is written, not added to, so m may move freely.
+        if (it == 0) {
+          m = mx;
+        } else {
+          // (True for a NaN too, which then reaches O and l.)
+          const bool grow = !((mx - m) * c2 <= kGrow) && mx != m;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float keep = grow ? ex2((m - mx) * c2) : 1.f;
+            if (grow) {
+              m = mx;
+              l *= keep;
+            }
+            if (!mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1)) return false;
+            tc_fence_after();
 #pragma unroll 1
-          for (int d = 0; d < D; d += 16) tmem_scale16(tO + quad + d, keep);
+            for (int d = 0; d < D; d += 16) tmem_scale16(tO + quad + d, keep);
+          }
         }
-      }
-      const float off = m == -INFINITY ? 0.f : m * c2;
-      const pair_t scale2 = pair(c2, c2), off2 = pair(-off, -off);
-      pair_t sums = pair(0.f, 0.f);
+        const float off = m == -INFINITY ? 0.f : m * c2;
+        const pair_t off2 = pair(-off, -off);
+        pair_t sums = pair(0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < kBN / 32; ++c) {
-        if (c * 32 >= nk) continue;
-        uint32_t w[16];
+        for (int c = 0; c < 2; ++c) {
+          if (!Whole && c * 32 >= nk) continue;
+          uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float2 x = split(fma2(pair(s[c][e], s[c][e + 1]), scale2, off2));
-          x = make_float2(ex2(x.x), ex2(x.y));
-          sums = add2(sums, pair(x.x, x.y));
-          w[e / 2] = Elem<T>::pack(x.x, x.y);
+          for (int e = 0; e < 32; e += 2) {
+            float2 x = split(fma2(pair(s[c][e], s[c][e + 1]), scale2, off2));
+            x = make_float2(ex2(x.x), ex2(x.y));
+            sums = add2(sums, pair(x.x, x.y));
+            w[e / 2] = Elem<T>::pack(x.x, x.y);
+          }
+          tmem_st16(tSt + c * 16, w);
         }
-        tmem_st16(tSt + c * 16, w);
-      }
-      const float2 halves = split(sums);
-      const float sum = halves.x + halves.y;
-      l += sum;
-      if (nk & 15) {
-        // Keys up to the next multiple of 16 have p = 0, but what V holds
-        // there (another event's rows) must not be able to make 0 * NaN.
-        const int st = it % Stages;
-        ok = mbar_wait(smem_addr(&sm.v_full[st]), (it / Stages) & 1);
-        if (!ok) break;
-        zero_tile_rows<Boxes, kBN>(sm.v[st], nk, (nk + 15) & ~15, threadIdx.x, 128);
-      }
-      tmem_wait_st();
+        const float2 halves = split(sums);
+        l += halves.x + halves.y;
+        if (!Whole && (nk & 15)) {
+          // Keys up to the next multiple of 16 have p = 0, but what V holds
+          // there (another event's rows) must not be able to make 0 * NaN.
+          const int st = n % Stages;
+          if (!mbar_wait(smem_addr(&sm.v_full[st]), (n / Stages) & 1)) return false;
+          zero_tile_rows<Boxes, kBN>(sm.v[st], nk, (nk + 15) & ~15, threadIdx.x, 128);
+        }
+        // O += P V of two tiles ago: long done, but waited for on every tile,
+        // so that the wait before a rescale can only mean the tile before.
+        if (n >= 2 && !mbar_wait(smem_addr(&sm.pv_done[n % 2]), (n / 2 - 1) & 1)) return false;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&sm.p_ready[n % 2]));
+        ++n;
+        return true;
+      };
+      const int whole = min(item.tiles, (p.causal ? min(t.len, t.i0 + 1) : t.len) / kBN);
+      int it = 0;
+      for (; it < whole && ok; ++it) ok = tile(std::true_type(), it);
+      for (; it < item.tiles && ok; ++it) ok = tile(std::false_type(), it);
+      if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1);
+      tc_fence_after();
+      const bool seen = i < t.len;
+      store_row<T>(seen ? row_ptr<T>(a.out, t, item.h, i) : nullptr, tO + quad, D,
+                   ok ? 1.f / l : NAN);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&sm.p_ready[it % 2]));
+      if (lane == 0) mbar_arrive(smem_addr(&sm.o_free));
+      if (seen)
+        a.lse[stat_at(p, t, p.heads, item.h, i)] = ok ? (m * c2 + log2f(l)) / kLog2e : NAN;
     }
-    if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(tiles - 1) % 2]), ((tiles - 1) / 2) & 1);
-    tc_fence_after();
-    const bool live = i < t.len;
-    store_row<T>(live ? row_ptr<T>(a.out, t, at.h, i) : nullptr, tO + quad, D,
-                 ok ? 1.f / l : NAN);
-    if (live) a.lse[stat_at(p, t, p.heads, at.h, i)] = ok ? (m * c2 + log2f(l)) / kLog2e : NAN;
     tc_fence_before();
   }
   __syncthreads();

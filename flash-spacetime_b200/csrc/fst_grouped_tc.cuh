@@ -284,7 +284,7 @@ __device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, i
 // The block's rows of no event: zeros, in 16-byte vectors, by n threads.
 template <typename T, int BM>
 __device__ __forceinline__ void zero_dead_rows(const FstRows& out, const RowTile& t, int h, int D,
-                                               int n) {
+                                               int n) {  // threads 0 to n - 1
   if (t.i0 + BM <= t.len) return;
   const int first = max(t.i0, t.len), rows = min(t.i0 + BM, t.lim) - first;
   for (int e = threadIdx.x; e < rows * (D / 8); e += n)
@@ -327,18 +327,100 @@ inline bool on_grid(const FstGroupedProblem& p, const FstRows& r, int heads) {
 }
 inline bool tc_type(const FstGroupedProblem& p) { return p.dtype != FST_F32 && p.head_dim % 8 == 0; }
 
+// ---- the feed of work --------------------------------------------------------
+//
+// A block stays on its SM and works through many positions of the grid. The
+// warp that feeds it asks the hardware for the next block that has not begun
+// (cluster launch control cancels that block's launch and returns its index),
+// looks its rows up in the work list, and hands them to the other warps
+// through two slots of shared memory, while those are still busy with the
+// positions before: the search, the launch and the first loads cost nothing
+// then, and the grid's order (heavy blocks first) and its balance are kept.
+
+struct Item {
+  RowTile t;
+  int h, kh;
+  int tiles;  // of the other side; 0: only rows of no event; below 0: the end
+};
+
+struct Feed {
+  alignas(16) uint4 answer;
+  Item item[2];
+  uint64_t full[2], empty[2], asked;
+};
+
+// One thread, before the block's barrier. `readers`: warps that take items.
+__device__ __forceinline__ void feed_init(Feed& f, int readers) {
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(smem_addr(&f.full[i]), 1);
+    mbar_init(smem_addr(&f.empty[i]), readers);
+  }
+  mbar_init(smem_addr(&f.asked), 1);
+}
+// Asks for another block's place, in the feeding warp's one thread.
+__device__ __forceinline__ void feed_ask(Feed& f) {
+  const uint32_t bar = smem_addr(&f.asked);
+  fence_proxy_async();  // the last answer has been read
+  mbar_arrive_tx(bar, 16);
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128"
+      " [%0], [%1];" ::"r"(smem_addr(&f.answer)),
+      "r"(bar)
+      : "memory");
+}
+// The answer to question number `round`: a block's index, or -1 (none is left;
+// nothing may be asked after that).
+__device__ __forceinline__ int feed_answer(Feed& f, int round) {
+  if (!mbar_wait(smem_addr(&f.asked), round & 1)) return -1;
+  int granted, x;
+  asm volatile(
+      "{\n .reg .b128 r;\n .reg .pred p;\n ld.shared.b128 r, [%2];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+      " selp.s32 %0, 1, 0, p;\n mov.s32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}"
+      : "=r"(granted), "=r"(x)
+      : "r"(smem_addr(&f.answer))
+      : "memory");
+  __syncwarp();  // read by all lanes before one of them asks again
+  return granted ? x : -1;
+}
+// A wait that may last as long as an item of `tiles` tiles takes.
+__device__ __forceinline__ bool wait_item(uint32_t bar, uint32_t parity, int tiles) {
+  for (int i = 0; i <= tiles / 1024; ++i)
+    if (mbar_wait(bar, parity)) return true;
+  return false;
+}
+// Hands over item number c (whole feeding warp); `tiles`: most tiles so far.
+__device__ __forceinline__ bool feed_put(Feed& f, int c, const Item& item, int tiles, int lane) {
+  if (c >= 2 && !wait_item(smem_addr(&f.empty[c % 2]), (c / 2 - 1) & 1, tiles)) return false;
+  if (lane == 0) {
+    f.item[c % 2] = item;
+    mbar_arrive(smem_addr(&f.full[c % 2]));
+  }
+  __syncwarp();
+  return true;
+}
+// Takes item number c (whole warps); false at the end.
+__device__ __forceinline__ bool feed_take(Feed& f, int c, Item& item, int lane) {
+  if (!mbar_wait(smem_addr(&f.full[c % 2]), (c / 2) & 1)) return false;
+  item = f.item[c % 2];
+  __syncwarp();
+  if (lane == 0) mbar_arrive(smem_addr(&f.empty[c % 2]));
+  return item.tiles >= 0;
+}
+
 // Head and work-list position of a block: key heads outermost (their K and V
 // stay in L2), the query heads of a group innermost (they share them).
 struct BlockAt {
   int kh, h, id;
 };
-__device__ __forceinline__ BlockAt block_at(const FstGroupedProblem& p, int blocks) {
+__device__ __forceinline__ BlockAt block_at(const FstGroupedProblem& p, int blocks, int index) {
   const int group = p.heads / p.kv_heads;
   BlockAt b;
-  const int x = blockIdx.x / group;
+  const int x = index / group;
   b.kh = x / blocks;
   b.id = x - b.kh * blocks;
-  b.h = b.kh * group + (blockIdx.x - x * group);
+  b.h = b.kh * group + (index - x * group);
   return b;
 }
 

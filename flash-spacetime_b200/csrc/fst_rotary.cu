@@ -2,10 +2,11 @@
 // k by position * freqs[pair], in one launch.
 //
 // One read and one write of every element is all it moves, so HBM is the
-// bound; the rest is arranged around that. A block takes a few rows (about
-// four 32-byte slots per thread) with all their heads, so the angles are
-// formed once per row and pair and shared by the heads through shared memory;
-// each thread issues its loads before the angles are formed.
+// bound; the rest keeps the instructions per element few. A thread owns one
+// slot (32 bytes) of a row and walks its heads: the cosines and sines of the
+// slot's pairs are formed once per row, shared by the block through shared
+// memory, and stay in the thread's registers for all heads. The first heads'
+// loads are issued before the angles are formed.
 //
 // The angle is position * freq, which for far positions reaches 1e6 rad and
 // more: fp32 would lose its phase. It is taken in turns in fp64,
@@ -19,18 +20,29 @@
 
 #include "fst_common.cuh"
 #include "fst_internal.h"
+#include "fst_tc_common.cuh"
 
 namespace fst {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kItems = 4;         // slots per thread and pass
-constexpr int kMaxRows = 16;      // rows per block
+// Measured at [21020, 32 + 8, 128] bf16 with 2 heads in flight and 10 heads a
+// thread, four blocks an SM: 79 us, 5.4 TB/s (4 in flight and 4 a thread,
+// three blocks: 91 us; 1 and 10, six blocks: 98 us).
+constexpr int kHeads = 2;         // heads of a thread in flight
+constexpr int kWalk = 10;         // heads of a thread
+constexpr int kMaxRows = 32;      // rows per block
 constexpr int kMaxTable = 2048;   // (cos, sin) pairs in shared memory
 
+// V channels as they are loaded and stored: 16 bytes, kept packed until they
+// are rotated, or one element.
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T x[V];
+struct Vec {
+  uint4 w;
+};
+template <typename T>
+struct Vec<T, 1> {
+  T w;
 };
 
 // A slot is two vectors of V channels, `a` and `b`: in a rotated slot of the
@@ -42,16 +54,16 @@ struct Slot {
   bool has_b;
 };
 
-template <int V>
+template <int V, bool Interleaved>
 __device__ __forceinline__ Slot slot_at(const FstRotaryArgs& p, int s) {
   Slot t;
-  const int rotated = p.interleaved ? (2 * p.pairs + 2 * V - 1) / (2 * V) : p.pairs / V;
-  if (!p.interleaved && s < rotated) {
+  const int rotated = Interleaved ? (2 * p.pairs + 2 * V - 1) / (2 * V) : p.pairs / V;
+  if (!Interleaved && s < rotated) {
     t.a = s * V;
     t.b = p.pairs + s * V;
     t.pair = s * V;
   } else {
-    t.a = p.interleaved ? s * 2 * V : 2 * p.pairs + (s - rotated) * 2 * V;
+    t.a = Interleaved ? s * 2 * V : 2 * p.pairs + (s - rotated) * 2 * V;
     t.b = t.a + V;
     t.pair = s < rotated ? t.a / 2 : -1;
   }
@@ -59,34 +71,51 @@ __device__ __forceinline__ Slot slot_at(const FstRotaryArgs& p, int s) {
   return t;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void rotate(const FstRotaryArgs& p, const Slot& t, const float2* cs,
-                                       Vec<T, V>& a, Vec<T, V>& b) {
-  if (t.pair < 0) return;
-  if (!p.interleaved || V == 1) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float2 c = cs[t.pair + e];
-      const float x = to_f<T>(a.x[e]), y = to_f<T>(b.x[e]);
-      a.x[e] = from_f<T>(x * c.x - y * c.y);
-      b.x[e] = from_f<T>(y * c.x + x * c.y);
-    }
+template <typename T>
+__device__ __forceinline__ float2 unpack(uint32_t w) {
+  return make_float2(tc::Elem<T>::lo(w), tc::Elem<T>::hi(w));
+}
+__device__ __forceinline__ float2 turn(float x, float y, float2 cs) {
+  return make_float2(x * cs.x - y * cs.y, y * cs.x + x * cs.y);
+}
+
+// Rotates a slot by cs, the cosines and sines of its V pairs: channel e of `a`
+// with channel e of `b`, or (Adjacent) neighbours within a and then b, up to
+// `left` pairs (an interleaved slot may reach past the rotated part).
+template <typename T, int V, bool Adjacent>
+__device__ __forceinline__ void rotate(const float2 (&cs)[V], int left, Vec<T, V>& a,
+                                       Vec<T, V>& b) {
+  if constexpr (V == 1) {
+    const float2 r = turn(to_f<T>(a.w), to_f<T>(b.w), cs[0]);
+    a.w = from_f<T>(r.x);
+    b.w = from_f<T>(r.y);
   } else {
-    // Pairs lie inside the vectors; the slot may reach past the rotated part.
+    uint32_t* wa = &a.w.x;
+    uint32_t* wb = &b.w.x;
 #pragma unroll
-    for (int e = 0; e + 1 < V; e += 2) {
-      const int pa = t.pair + e / 2, pb = pa + V / 2;
-      if (pa < p.pairs) {
-        const float2 c = cs[pa];
-        const float x = to_f<T>(a.x[e]), y = to_f<T>(a.x[e + 1]);
-        a.x[e] = from_f<T>(x * c.x - y * c.y);
-        a.x[e + 1] = from_f<T>(y * c.x + x * c.y);
-      }
-      if (pb < p.pairs) {
-        const float2 c = cs[pb];
-        const float x = to_f<T>(b.x[e]), y = to_f<T>(b.x[e + 1]);
-        b.x[e] = from_f<T>(x * c.x - y * c.y);
-        b.x[e + 1] = from_f<T>(y * c.x + x * c.y);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (Adjacent && sizeof(T) == 2) {
+        const float2 x = unpack<T>(wa[i]), y = unpack<T>(wb[i]);
+        const float2 u = turn(x.x, x.y, cs[i]), v = turn(y.x, y.y, cs[4 + i]);
+        if (i < left) wa[i] = tc::Elem<T>::pack(u.x, u.y);
+        if (4 + i < left) wb[i] = tc::Elem<T>::pack(v.x, v.y);
+      } else if constexpr (Adjacent) {
+        uint32_t* w = i < 2 ? wa : wb;
+        const int n = i % 2 * 2;
+        const float2 u = turn(__uint_as_float(w[n]), __uint_as_float(w[n + 1]), cs[i]);
+        if (i < left) {
+          w[n] = __float_as_uint(u.x);
+          w[n + 1] = __float_as_uint(u.y);
+        }
+      } else if constexpr (sizeof(T) == 2) {
+        const float2 x = unpack<T>(wa[i]), y = unpack<T>(wb[i]);
+        const float2 u = turn(x.x, y.x, cs[2 * i]), v = turn(x.y, y.y, cs[2 * i + 1]);
+        wa[i] = tc::Elem<T>::pack(u.x, v.x);
+        wb[i] = tc::Elem<T>::pack(u.y, v.y);
+      } else {
+        const float2 u = turn(__uint_as_float(wa[i]), __uint_as_float(wb[i]), cs[i]);
+        wa[i] = __float_as_uint(u.x);
+        wb[i] = __float_as_uint(u.y);
       }
     }
   }
@@ -115,87 +144,91 @@ __device__ __forceinline__ bool position_of(const FstRotaryArgs& p, int64_t row,
   return true;
 }
 
-// Quotients of a block's item numbers: n / d = umulhi(n, ceil(2^32 / d)) while
-// n d < 2^32, which the host makes sure of (a 32-bit division would cost more
-// instructions than the rotation).
-struct Split {
-  int rows_per_block, heads, slots;
-  uint32_t by_heads, by_slots;  // 0: the divisor is 1
+// How a block's threads share its rows: thread u is slot u % slots, head group
+// u / slots % groups, row u / slots / groups, and takes every groups-th head.
+struct Shape {
+  int rows, groups, heads, slots;
 };
-__device__ __forceinline__ int quotient(int n, uint32_t by) {
-  return by ? (int)__umulhi((uint32_t)n, by) : n;
-}
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(FstRotaryArgs p, Split sp) {
-  __shared__ float2 cs[kMaxTable];
+template <typename T, int V, bool Interleaved>
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(FstRotaryArgs p, Shape sh) {
+  __shared__ float2 table[kMaxTable];
   __shared__ double pos[kMaxRows];
   __shared__ int live[kMaxRows];
-  const int64_t row0 = (int64_t)blockIdx.x * sp.rows_per_block;
-  const int rows = (int)min((int64_t)sp.rows_per_block, p.total_rows - row0);
+  const int64_t row0 = (int64_t)blockIdx.x * sh.rows;
+  const int rows = (int)min((int64_t)sh.rows, p.total_rows - row0);
   // Padded: event and row of the block's first row.
   const int64_t ev0 = p.packed ? 0 : row0 / p.max_len;
   const int64_t i0 = p.packed ? row0 : row0 - ev0 * p.max_len;
   using W = Vec<T, V>;
-  const int items = rows * sp.heads * sp.slots;  // host: below 2^31
-  for (int base = 0; base < items; base += kThreads * kItems) {
-    W a[kItems], b[kItems];
-    T* dst[kItems];
-    int where[kItems];  // row of the block and slot of the head
-#pragma unroll
-    for (int n = 0; n < kItems; ++n) {
-      const int item = base + n * kThreads + threadIdx.x;
-      dst[n] = nullptr;
-      if (item >= items) continue;
-      const int rh = quotient(item, sp.by_slots), s = item - rh * sp.slots;
-      const int r = quotient(rh, sp.by_heads), h = rh - r * sp.heads;
-      where[n] = r << 16 | s;  // slots: at most 1024 / 2 + 1
-      const Slot t = slot_at<V>(p, s);
-      int64_t ev = ev0, i = i0 + r;
-      while (!p.packed && i >= p.max_len) {
-        i -= p.max_len;
-        ++ev;
-      }
-      const bool is_k = h >= p.heads;
-      const FstRows& in = is_k ? p.k : p.q;
-      const FstRows& out = is_k ? p.k_out : p.q_out;
-      const int hh = is_k ? h - p.heads : h;
-      const T* src =
-          (const T*)in.data + ev * in.event_stride + i * in.row_stride + hh * in.head_stride;
-      dst[n] = (T*)out.data + ev * out.event_stride + i * out.row_stride + hh * out.head_stride;
-      a[n] = *(const W*)(src + t.a);
-      if (t.has_b) b[n] = *(const W*)(src + t.b);
+  const int units = rows * sh.groups * sh.slots;
+  bool formed = false;
+  for (int u0 = 0; u0 < units; u0 += kThreads) {
+    const int u = u0 + threadIdx.x, gr = u / sh.slots, r = gr / sh.groups;
+    const int g = gr - r * sh.groups;
+    const bool mine = u < units;
+    const Slot t = slot_at<V, Interleaved>(p, u - gr * sh.slots);
+    int64_t ev = ev0, i = i0 + r;
+    while (mine && !p.packed && i >= p.max_len) {
+      i -= p.max_len;
+      ++ev;
     }
-    if (base == 0) {
-      // The angles, while the loads are on their way.
-      if (threadIdx.x < rows) {
-        const int64_t at = row0 + threadIdx.x;
-        int64_t count = 0;
-        live[threadIdx.x] =
-            position_of(p, at, p.packed ? at : (i0 + threadIdx.x) % p.max_len, count);
-        pos[threadIdx.x] = (double)count;
+    const T* q = (const T*)p.q.data + ev * p.q.event_stride + i * p.q.row_stride;
+    const T* k = (const T*)p.k.data + ev * p.k.event_stride + i * p.k.row_stride;
+    T* q_out = (T*)p.q_out.data + ev * p.q_out.event_stride + i * p.q_out.row_stride;
+    T* k_out = (T*)p.k_out.data + ev * p.k_out.event_stride + i * p.k_out.row_stride;
+    W a[kHeads], b[kHeads];
+    float2 cs[V];
+    for (int h0 = g; h0 < sh.heads || !formed; h0 += kHeads * sh.groups) {
+#pragma unroll
+      for (int n = 0; n < kHeads; ++n) {
+        const int h = h0 + n * sh.groups;
+        if (!mine || h >= sh.heads) continue;
+        const T* src = h < p.heads ? q + h * p.q.head_stride
+                                   : k + (h - p.heads) * p.k.head_stride;
+        a[n] = *(const W*)(src + t.a);
+        if (t.has_b) b[n] = *(const W*)(src + t.b);
       }
-      __syncthreads();
-      for (int e = threadIdx.x; e < rows * p.pairs; e += kThreads) {
-        const int r = e / p.pairs;
-        float sn = 0.f, c = 1.f;
-        if (live[r]) {
-          const double t = pos[r] * (p.freqs[e - r * p.pairs] * 0.15915494309189533577);
-          sincospif((float)(2.0 * (t - rint(t))), &sn, &c);
-          sn *= p.inverse ? -p.magnitude : p.magnitude;
-          c *= p.magnitude;
+      if (!formed) {
+        // The angles, while the loads are on their way.
+        formed = true;
+        if (threadIdx.x < rows) {
+          const int64_t at = row0 + threadIdx.x;
+          int64_t count = 0;
+          live[threadIdx.x] =
+              position_of(p, at, p.packed ? at : (i0 + threadIdx.x) % p.max_len, count);
+          pos[threadIdx.x] = (double)count;
         }
-        cs[e] = make_float2(c, sn);
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * p.pairs; e += kThreads) {
+          const int er = e / p.pairs;
+          float sn = 0.f, c = 1.f;
+          if (live[er]) {
+            const double turns = pos[er] * (p.freqs[e - er * p.pairs] * 0.15915494309189533577);
+            sincospif((float)(2.0 * (turns - rint(turns))), &sn, &c);
+            sn *= p.inverse ? -p.magnitude : p.magnitude;
+            c *= p.magnitude;
+          }
+          table[e] = make_float2(c, sn);
+        }
+        __syncthreads();
       }
-      __syncthreads();
-    }
+      if (!mine) continue;
+      if (h0 == g && t.pair >= 0) {
 #pragma unroll
-    for (int n = 0; n < kItems; ++n) {
-      if (!dst[n]) continue;
-      const Slot t = slot_at<V>(p, where[n] & 0xffff);
-      rotate<T, V>(p, t, cs + (where[n] >> 16) * p.pairs, a[n], b[n]);
-      *(W*)(dst[n] + t.a) = a[n];
-      if (t.has_b) *(W*)(dst[n] + t.b) = b[n];
+        for (int e = 0; e < V; ++e)
+          cs[e] = t.pair + e < p.pairs ? table[r * p.pairs + t.pair + e] : make_float2(1.f, 0.f);
+      }
+#pragma unroll
+      for (int n = 0; n < kHeads; ++n) {
+        const int h = h0 + n * sh.groups;
+        if (h >= sh.heads) continue;
+        if (t.pair >= 0) rotate<T, V, Interleaved && V != 1>(cs, p.pairs - t.pair, a[n], b[n]);
+        T* dst = h < p.heads ? q_out + h * p.q_out.head_stride
+                             : k_out + (h - p.heads) * p.k_out.head_stride;
+        *(W*)(dst + t.a) = a[n];
+        if (t.has_b) *(W*)(dst + t.b) = b[n];
+      }
     }
   }
 }
@@ -218,24 +251,22 @@ int launch(const FstRotaryArgs& p, cudaStream_t st) {
   const int slots = p.interleaved ? (p.head_dim + 2 * w - 1) / (2 * w)
                                   : rot + (p.head_dim - 2 * p.pairs + 2 * w - 1) / (2 * w);
   const int heads = p.heads + (p.k.data ? p.kv_heads : 0);
-  const int64_t row_items = (int64_t)heads * slots;
-  int64_t rows = kThreads * kItems / row_items;
+  // kWalk heads a thread where there are as many, and as many rows as fill
+  // the block.
+  int groups = (heads + kWalk - 1) / kWalk;
+  if (groups * (int64_t)slots > kThreads) groups = slots < kThreads ? kThreads / slots : 1;
+  int rows = kThreads / (groups * slots);
   if (rows > kMaxRows) rows = kMaxRows;
   if (p.pairs > 0 && rows > kMaxTable / p.pairs) rows = kMaxTable / p.pairs;
   if (rows < 1) rows = 1;
-  if (row_items >= (1ll << 31) ||
-      rows * row_items * (heads > slots ? heads : slots) >= (1ll << 32))
-    return api_fail(FST_ERR_UNSUPPORTED, "rotary: %d heads of %d are too many", heads, p.head_dim);
   const int64_t blocks = (p.total_rows + rows - 1) / rows;
   if (blocks >= (1ll << 31))
     return api_fail(FST_ERR_UNSUPPORTED, "rotary: %lld rows are too many",
                     (long long)p.total_rows);
-  auto by = [](int d) { return d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u; };
-  const Split sp{(int)rows, heads, slots, by(heads), by(slots)};
-  if (vec)
-    rotary_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(p, sp);
-  else
-    rotary_kernel<T, 1><<<(unsigned)blocks, kThreads, 0, st>>>(p, sp);
+  const Shape sh{rows, groups, heads, slots};
+  const auto kernel = vec ? (p.interleaved ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>)
+                          : (p.interleaved ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
+  kernel<<<(unsigned)blocks, kThreads, 0, st>>>(p, sh);
   count_launch();
   return FST_OK;
 }
