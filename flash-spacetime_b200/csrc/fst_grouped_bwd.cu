@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "fst_grouped_tc.cuh"
 
@@ -181,17 +182,15 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       }
     }
     const pair_t scale2 = pair(c2, c2), lse2n = pair(-lse2, -lse2), delta2n = pair(-delta, -delta);
-    for (int it = 0; it < tiles; ++it) {
+    // One tile. `Whole`: every row of the block sees all its keys.
+    auto tile = [&](auto whole, int it) {
+      constexpr bool Whole = decltype(whole)::value;
       const int j0 = it * kBN + w * 64, nk = end - j0;
-      const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
-      const bool edge = j0 + 64 > t.len || (p.causal && j0 + 64 > t.i0 + 1);
-      ok = mbar_wait(smem_addr(&sm.s_full), it & 1);
-      if (!ok) break;
+      if (!mbar_wait(smem_addr(&sm.s_full), it & 1)) return false;
       tc_fence_after();
       float s[2][32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (c * 32 < nk) tmem_ld32(s[c], tS + c * 32);
+      if (Whole || nk > 0) tmem_ld32(s[0], tS);
+      if (Whole || nk > 32) tmem_ld32(s[1], tS + 32);
       tmem_wait_ld();
       pin(s[0]);
       pin(s[1]);
@@ -199,19 +198,20 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&sm.s_free));
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float2 x = split(fma2(pair(s[c][e], s[c][e + 1]), scale2, lse2n));
-          s[c][e] = ex2(x.x);
-          s[c][e + 1] = ex2(x.y);
-        }
-      ok = mbar_wait(smem_addr(&sm.dp_full), it & 1);
-      if (!ok) break;
+      for (int e = 0; e < 64; e += 2) {
+        float* x = &s[e / 32][e % 32];
+        const float2 y = split(fma2(pair(x[0], x[1]), scale2, lse2n));
+        x[0] = ex2(y.x);
+        x[1] = ex2(y.y);
+      }
+      if (!mbar_wait(smem_addr(&sm.dp_full), it & 1)) return false;
       tc_fence_after();
+      // Keys below lim are seen; the warp's first row sees fewest.
+      const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
+      const int fewest = Whole ? 64 : uniform(lim);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        if (c * 32 >= nk) continue;
+        if (!Whole && c * 32 >= nk) continue;
         float dp[32];
         tmem_ld32(dp, tP + c * 32);
         tmem_wait_ld();
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
           dp[e] = x.x;
           dp[e + 1] = x.y;
         }
-        if (edge) {
+        if (!Whole && c * 32 + 32 > fewest) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) dp[e] = c * 32 + e < lim ? dp[e] : 0.f;
         }
@@ -233,13 +233,18 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         tmem_st16(tP + c * 16, x);
       }
       const int all = min(kBN, end - it * kBN);
-      if (all & 15)  // dS is 0 there, and must not meet another event's NaN
+      if (!Whole && (all & 15))  // dS is 0 there, and must not meet another event's NaN
         zero_tile_rows<Boxes, kBN>(sm.k[it % Stages], all, (all + 15) & ~15, threadIdx.x, W * 128);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&sm.ds_ready));
-    }
+      return true;
+    };
+    const int whole = min(tiles, (p.causal ? min(t.len, t.i0 + 1) : t.len) / kBN);
+    int it = 0;
+    for (; it < whole && ok; ++it) ok = tile(std::true_type(), it);
+    for (; it < tiles && ok; ++it) ok = tile(std::false_type(), it);
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
     // The groups share the columns of the result.

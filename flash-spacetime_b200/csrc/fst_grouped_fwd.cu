@@ -83,14 +83,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   const uint32_t tS = tmem, tO = tmem + 128;
-  // Two blocks that begin together would ask for the exponentials, and for the
-  // tensor cores, at the same time all along: the one in the upper half of
-  // tensor memory starts half a tile later.
-  if (tmem & 256) {
-    const uint32_t start = (uint32_t)clock();
-    while ((uint32_t)clock() - start < 600) {
-    }
-  }
+  stagger(tmem, 600);
 
   // Barriers and buffers go by the tile's number n in the block's life; `live`
   // counts its items that have tiles.
