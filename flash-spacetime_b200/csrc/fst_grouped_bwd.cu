@@ -50,6 +50,7 @@ struct RowSmem {
   alignas(1024) char g[Boxes * kBM * 128];
   alignas(1024) char k[Stages][Boxes * W * 64 * 128];
   alignas(1024) char v[Stages][Boxes * W * 64 * 128];
+  float delta[2][kBM];  // the groups' shares of D
   uint64_t own_full, full[Stages], empty[Stages], s_full, s_free, dp_full, ds_ready, done;
   uint32_t tmem;
 };
@@ -165,15 +166,30 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const float c2 = fabsf(p.scale) * kLog2e;
     float lse2 = 0.f, delta = 0.f;
     if (live) {
-      const T* o = row_ptr<T>(a.out, t, at.h, i);
-      const T* g = row_ptr<T>(a.dout, t, at.h, i);
-      for (int d = 0; d < D; d += 8) {
-        const uint4 x = *(const uint4*)(o + d), y = *(const uint4*)(g + d);
-        delta += Elem<T>::lo(x.x) * Elem<T>::lo(y.x) + Elem<T>::hi(x.x) * Elem<T>::hi(y.x);
-        delta += Elem<T>::lo(x.y) * Elem<T>::lo(y.y) + Elem<T>::hi(x.y) * Elem<T>::hi(y.y);
-        delta += Elem<T>::lo(x.z) * Elem<T>::lo(y.z) + Elem<T>::hi(x.z) * Elem<T>::hi(y.z);
-        delta += Elem<T>::lo(x.w) * Elem<T>::lo(y.w) + Elem<T>::hi(x.w) * Elem<T>::hi(y.w);
+      // Each group sums its 64 channels.
+      const int d0 = w * 64, n = W == 1 ? D : min(D - d0, 64);
+      const T* g = row_ptr<T>(a.dout, t, at.h, i) + d0;
+      const T* o = row_ptr<T>(a.out, t, at.h, i) + d0;
+      const T* r = a.out_low.data ? row_ptr<T>(a.out_low, t, at.h, i) + d0 : nullptr;
+#pragma unroll 4
+      for (int d = 0; d < n; d += 8) {
+        const uint4 y = *(const uint4*)(g + d), x = *(const uint4*)(o + d);
+        const uint4 z = r ? *(const uint4*)(r + d) : make_uint4(0, 0, 0, 0);
+        const uint32_t ys[4] = {y.x, y.y, y.z, y.w}, xs[4] = {x.x, x.y, x.z, x.w},
+                       zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          delta = fmaf(Elem<T>::lo(xs[e]) + Elem<T>::lo(zs[e]), Elem<T>::lo(ys[e]), delta);
+          delta = fmaf(Elem<T>::hi(xs[e]) + Elem<T>::hi(zs[e]), Elem<T>::hi(ys[e]), delta);
+        }
       }
+    }
+    if (W == 2) {
+      sm.delta[w][row] = delta;
+      tc::named_sync(1, W * 128);
+      delta = sm.delta[0][row] + sm.delta[1][row];
+    }
+    if (live) {
       const int64_t st = stat_at(p, t, p.heads, at.h, i);
       lse2 = a.lse[st] * kLog2e;
       if (w == 0) {  // for the column kernel, in the form it adds them
@@ -248,7 +264,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
     // The groups share the columns of the result.
-    store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr,
+    store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr, nullptr,
                  tmem + quad + 2 * kBN + w * 64, W == 1 ? D : min(D - w * 64, 64),
                  ok ? p.scale : NAN);
     tc_fence_before();
@@ -500,9 +516,10 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const bool live = j < t.len;
     const uint32_t tV = tmem + quad + 2 * kBN, tK = tV + kAcc;
     if (w == 0)
-      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, tV, D, ok ? 1.f : NAN);
+      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, nullptr, tV, D, ok ? 1.f : NAN);
     if (w == W - 1)
-      store_row<T>(live ? row_ptr<T>(a.dk, t, kh, j) : nullptr, tK, D, ok ? p.scale : NAN);
+      store_row<T>(live ? row_ptr<T>(a.dk, t, kh, j) : nullptr, nullptr, tK, D,
+                   ok ? p.scale : NAN);
     tc_fence_before();
   }
   __syncthreads();
@@ -558,7 +575,7 @@ int launch_t(const FstGroupedBackwardArgs& a, cudaStream_t st) {
 bool tc_takes(const FstGroupedBackwardArgs& a) {
   const FstGroupedProblem& p = a.prob;
   return tc_type(p) && on_grid(p, a.q, p.heads) && on_grid(p, a.out, p.heads) &&
-         on_grid(p, a.dout, p.heads) && on_grid(p, a.dq, p.heads) &&
+         (!a.out_low.data || on_grid(p, a.out_low, p.heads)) && on_grid(p, a.dout, p.heads) && on_grid(p, a.dq, p.heads) &&
          on_grid(p, a.k, p.kv_heads) && on_grid(p, a.v, p.kv_heads) &&
          on_grid(p, a.dk, p.kv_heads) && on_grid(p, a.dv, p.kv_heads);
 }

@@ -284,8 +284,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1);
       tc_fence_after();
       const bool seen = i < t.len;
-      store_row<T>(seen ? row_ptr<T>(a.out, t, item.h, i) : nullptr, tO + quad, D,
-                   ok ? 1.f / l : NAN);
+      store_row<T>(seen ? row_ptr<T>(a.out, t, item.h, i) : nullptr,
+                   seen && a.out_low.data ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr,
+                   tO + quad, D, ok ? 1.f / l : NAN);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&sm.o_free));
@@ -331,6 +332,7 @@ int launch_t(const FstGroupedForwardArgs& a, cudaStream_t st) {
 bool tc_takes(const FstGroupedForwardArgs& a) {
   const FstGroupedProblem& p = a.prob;
   return tc_type(p) && on_grid(p, a.q, p.heads) && on_grid(p, a.out, p.heads) &&
+         (!a.out_low.data || on_grid(p, a.out_low, p.heads)) &&
          on_grid(p, a.k, p.kv_heads) && on_grid(p, a.v, p.kv_heads);
 }
 

@@ -186,6 +186,18 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(FstGroupedForwardArgs a) 
       a.lse[stat_at(p, t, p.heads, h, i)] = (m[r] + log2f(l[r])) / kLog2e;
   }
   store_rows<T, DM>(a.out, t, h, D, ty, tx, acc, inv);
+  if (a.out_low.data) {
+    // What rounding to T left over.
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < DM / 16; ++c) {
+        const float x = acc[r][c] * inv[r];
+        acc[r][c] = x - to_f<T>(from_f<T>(x));
+      }
+    const float one[4] = {1.f, 1.f, 1.f, 1.f};
+    store_rows<T, DM>(a.out_low, t, h, D, ty, tx, acc, one);
+  }
 }
 
 // dq, and D_i = dO_i . o_i for the dk / dv kernel.
@@ -207,6 +219,9 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(FstGroupedBackwardArgs a) 
   load_tile<T, DM>(Q, row_ptr<T>(a.q, t, h, t.i0), a.q.row_stride, t.len - t.i0, D);
   load_tile<T, DM>(G, row_ptr<T>(a.dout, t, h, t.i0), a.dout.row_stride, t.len - t.i0, D);
   load_tile<T, DM>(K, row_ptr<T>(a.out, t, h, t.i0), a.out.row_stride, t.len - t.i0, D);
+  const bool low = a.out_low.data != nullptr;
+  if (low)
+    load_tile<T, DM>(V, row_ptr<T>(a.out_low, t, h, t.i0), a.out_low.row_stride, t.len - t.i0, D);
   __syncthreads();
   const float c2 = p.scale * kLog2e;
   float lse2[4], delta[4], acc[4][DM / 16] = {};
@@ -215,7 +230,10 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(FstGroupedBackwardArgs a) 
     const int i = t.i0 + 4 * ty + r;
     float sum = 0.f;
     for (int d = tx; d < DM; d += 16)
-      sum = fmaf(G[(4 * ty + r) * (DM + 4) + d], K[(4 * ty + r) * (DM + 4) + d], sum);
+    {
+      const int at = (4 * ty + r) * (DM + 4) + d;
+      sum = fmaf(G[at], low ? K[at] + V[at] : K[at], sum);
+    }
     delta[r] = half_warp_sum(sum);
     const int64_t at = stat_at(p, t, p.heads, h, i);
     lse2[r] = i < t.len ? a.lse[at] * kLog2e : 0.f;

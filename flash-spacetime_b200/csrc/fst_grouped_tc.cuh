@@ -305,9 +305,9 @@ __device__ __forceinline__ void zero_dead_rows(const FstRows& out, const RowTile
 }
 
 // A thread's row of D accumulator columns, times f, rounded and stored (whole
-// warps; out may be null).
+// warps; out may be null). What the rounding left over goes to `low`, if any.
 template <typename T>
-__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f) {
+__device__ __forceinline__ void store_row(T* out, T* low, uint32_t acc, int D, float f) {
   for (int d = 0; d < D; d += 32) {
     float o[32];
     tmem_ld32(o, acc + d);
@@ -316,12 +316,15 @@ __device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f) 
 #pragma unroll
     for (int e = 0; e < 32; e += 8) {
       if (!out || d + e >= D) break;
-      uint4 w;
-      w.x = Elem<T>::pack(o[e] * f, o[e + 1] * f);
-      w.y = Elem<T>::pack(o[e + 2] * f, o[e + 3] * f);
-      w.z = Elem<T>::pack(o[e + 4] * f, o[e + 5] * f);
-      w.w = Elem<T>::pack(o[e + 6] * f, o[e + 7] * f);
-      *(uint4*)(out + d + e) = w;
+      uint32_t w[4], r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = o[e + 2 * i] * f, y = o[e + 2 * i + 1] * f;
+        w[i] = Elem<T>::pack(x, y);
+        r[i] = Elem<T>::pack(x - Elem<T>::lo(w[i]), y - Elem<T>::hi(w[i]));
+      }
+      *(uint4*)(out + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (low) *(uint4*)(low + d + e) = make_uint4(r[0], r[1], r[2], r[3]);
     }
     __syncwarp();  // tcgen05.ld takes the whole warp
   }

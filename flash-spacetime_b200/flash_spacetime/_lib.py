@@ -143,6 +143,7 @@ class FstGroupedForwardArgs(ctypes.Structure):
         ("k", FstRows),
         ("v", FstRows),
         ("out", FstRows),
+        ("out_low", FstRows),
         ("lse", ctypes.c_void_p),
     ]
 
@@ -154,6 +155,7 @@ class FstGroupedBackwardArgs(ctypes.Structure):
         ("k", FstRows),
         ("v", FstRows),
         ("out", FstRows),
+        ("out_low", FstRows),
         ("dout", FstRows),
         ("dq", FstRows),
         ("dk", FstRows),

@@ -15,6 +15,10 @@ Conventions:
   and are exactly 0 in the output and in every gradient;
 * softmax statistics and sums are fp32; results are bitwise deterministic run
   to run (no atomics);
+* with gradients, a 16-bit forward also keeps what rounding its output left
+  over, so that the backward's row sums ``D = dO . out`` are those of the
+  unrounded output: rows of few keys would otherwise carry its rounding into
+  dq and dk;
 * inputs are read in place whatever their strides, as long as the channels of
   a head are adjacent: slices of a fused projection need no copy.
 """
@@ -34,8 +38,9 @@ from .ops import _DTYPES, _padded_lengths, _timed_call
 # FstRows is (data, event, head, row stride).
 _PROBLEM = "8iqfi2Q"
 _ROWS = "Q3q"
-_FORWARD = struct.Struct("@" + _PROBLEM + 4 * _ROWS + "Q")
-_BACKWARD = struct.Struct("@" + _PROBLEM + 8 * _ROWS + "2Q")
+_FORWARD = struct.Struct("@" + _PROBLEM + 5 * _ROWS + "Q")
+_BACKWARD = struct.Struct("@" + _PROBLEM + 9 * _ROWS + "2Q")
+_NO_ROWS = (0, 0, 0, 0)
 _CONTIGUOUS = torch.contiguous_format
 
 Sizes = Tuple[int, int, int, int]
@@ -131,33 +136,36 @@ def _problem(q: Tensor, kv_heads: int, layout: str, lens: Tensor, scale: float,
 
 
 def _forward(q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str, scale: float,
-             causal: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """One ``fst_grouped_forward`` call: out, lse, and q, k, v as read."""
+             causal: bool, keep_low: bool = False) -> Tuple[Any, ...]:
+    """One ``fst_grouped_forward`` call: out, lse, q, k, v as read, and with
+    ``keep_low`` what rounding a 16-bit out left over (else None)."""
     q, k, v = _in_place(q), _in_place(k), _in_place(v)
     events, rows, heads, _ = _shape(q, layout, "q")
     out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    low = torch.empty_like(out) if keep_low and q.element_size() == 2 else None
     shape = (heads, rows) if layout == "packed" else (events, heads, rows)
     lse = torch.empty(shape, dtype=torch.float32, device=q.device)
     args = _FORWARD.pack(
         *_problem(q, _shape(k, layout, "k")[2], layout, lens, scale, causal), *_rows(q, layout),
-        *_rows(k, layout), *_rows(v, layout), *_rows(out, layout), lse.data_ptr())
+        *_rows(k, layout), *_rows(v, layout), *_rows(out, layout),
+        *(_NO_ROWS if low is None else _rows(low, layout)), lse.data_ptr())
     _call("fst_grouped_forward", args, q.device)
-    return out, lse, q, k, v
+    return out, lse, q, k, v, low
 
 
 class _FlashGroupedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str,
                 scale: float, causal: bool) -> Tensor:  # type: ignore[override]
-        out, lse, q, k, v = _forward(q, k, v, lens, layout, scale, causal)
-        ctx.save_for_backward(q, k, v, out, lse, lens)
+        out, lse, q, k, v, low = _forward(q, k, v, lens, layout, scale, causal, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, lens)
         ctx.layout, ctx.scale, ctx.causal = layout, scale, causal
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad_out: Tensor) -> Tuple[Optional[Tensor], ...]:  # type: ignore[override]
-        q, k, v, out, lse, lens = ctx.saved_tensors
+        q, k, v, out, low, lse, lens = ctx.saved_tensors
         layout = ctx.layout
         dout = _in_place(grad_out)
         dq, dk, dv = (torch.empty_like(t, memory_format=_CONTIGUOUS) for t in (q, k, v))
@@ -165,8 +173,8 @@ class _FlashGroupedAttention(torch.autograd.Function):
         args = _BACKWARD.pack(
             *_problem(q, _shape(k, layout, "k")[2], layout, lens, ctx.scale, ctx.causal),
             *_rows(q, layout), *_rows(k, layout), *_rows(v, layout), *_rows(out, layout),
-            *_rows(dout, layout), *_rows(dq, layout), *_rows(dk, layout), *_rows(dv, layout),
-            lse.data_ptr(), stats.data_ptr())
+            *(_NO_ROWS if low is None else _rows(low, layout)), *_rows(dout, layout),
+            *_rows(dq, layout), *_rows(dk, layout), *_rows(dv, layout), lse.data_ptr(), stats.data_ptr())
         _call("fst_grouped_backward", args, q.device)
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,

@@ -14,11 +14,10 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from .grouped import _CONTIGUOUS, _ROWS, _call, _check_tensor, _integers, _rows, _shape
+from .grouped import _CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _integers, _rows, _shape
 from .ops import _DTYPES
 
 _ROTARY = struct.Struct("@11ifq3Q" + 4 * _ROWS)
-_NO_ROWS = (0, 0, 0, 0)
 
 
 def _adjacent(t: Tensor) -> Tensor:

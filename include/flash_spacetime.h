@@ -278,6 +278,8 @@ typedef struct FstGroupedForwardArgs {
   FstRows k;             /* Hkv heads                                        */
   FstRows v;
   FstRows out;           /* output, H heads                                  */
+  FstRows out_low;       /* output or data NULL: what rounding out to its    */
+                         /* type left over, in that type (16-bit types only) */
   float* lse;            /* output                                           */
 } FstGroupedForwardArgs;
 
@@ -287,6 +289,8 @@ typedef struct FstGroupedBackwardArgs {
   FstRows k;
   FstRows v;
   FstRows out;           /* forward output                                   */
+  FstRows out_low;       /* forward output or data NULL: with it D_i = dout_i . */
+                         /* out_i keeps the rows of few keys exact           */
   FstRows dout;          /* its gradient; padding rows ignored               */
   FstRows dq;            /* outputs                                          */
   FstRows dk;

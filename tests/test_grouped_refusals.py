@@ -48,11 +48,11 @@ def test_packed_argument_formats_have_the_struct_sizes():
                      (rotary._ROTARY, _lib.FstRotaryArgs)):
         assert fmt.size == ctypes.sizeof(cls)
     # Field by field: distinct values in, the same out of the ctypes mirror.
-    a = _lib.FstGroupedForwardArgs.from_buffer_copy(grouped._FORWARD.pack(*range(1, 31)))
+    a = _lib.FstGroupedForwardArgs.from_buffer_copy(grouped._FORWARD.pack(*range(1, 35)))
     assert [getattr(a.prob, f) for f, _ in a.prob._fields_] == list(range(1, 14))
-    assert (a.q.data, a.q.row_stride, a.out.event_stride, a.lse) == (14, 17, 27, 30)
-    b = _lib.FstGroupedBackwardArgs.from_buffer_copy(grouped._BACKWARD.pack(*range(1, 48)))
-    assert (b.dout.data, b.dv.row_stride, b.lse, b.stats) == (30, 45, 46, 47)
+    assert (a.q.data, a.q.row_stride, a.out_low.event_stride, a.lse) == (14, 17, 31, 34)
+    b = _lib.FstGroupedBackwardArgs.from_buffer_copy(grouped._BACKWARD.pack(*range(1, 52)))
+    assert (b.dout.data, b.dv.row_stride, b.lse, b.stats) == (34, 49, 50, 51)
     r = _lib.FstRotaryArgs.from_buffer_copy(rotary._ROTARY.pack(*range(1, 33)))
     assert [getattr(r, f) for f, _ in r._fields_[:16]] == list(range(1, 17))
     assert (r.q.data, r.k_out.row_stride) == (17, 32)
