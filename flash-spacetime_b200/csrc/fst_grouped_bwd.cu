@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
     // The groups share the columns of the result.
-    store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr, nullptr,
+    store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr,
                  tmem + quad + 2 * kBN + w * 64, W == 1 ? D : min(D - w * 64, 64),
                  ok ? p.scale : NAN);
     tc_fence_before();
@@ -516,9 +516,9 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const bool live = j < t.len;
     const uint32_t tV = tmem + quad + 2 * kBN, tK = tV + kAcc;
     if (w == 0)
-      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, nullptr, tV, D, ok ? 1.f : NAN);
+      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, tV, D, ok ? 1.f : NAN);
     if (w == W - 1)
-      store_row<T>(live ? row_ptr<T>(a.dk, t, kh, j) : nullptr, nullptr, tK, D,
+      store_row<T>(live ? row_ptr<T>(a.dk, t, kh, j) : nullptr, tK, D,
                    ok ? p.scale : NAN);
     tc_fence_before();
   }

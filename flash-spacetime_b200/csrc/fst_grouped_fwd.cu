@@ -83,7 +83,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   const uint32_t tS = tmem, tO = tmem + 128;
-  stagger(tmem, 600);
+  // Two blocks of an SM that begin together would ask for the exponentials, and
+  // for the tensor cores, at the same time all along: the one whose columns are
+  // the upper half of tensor memory starts half a tile later.
+  if (tmem & 256) {
+    const uint32_t start = (uint32_t)clock();
+    while ((uint32_t)clock() - start < 600) {
+    }
+  }
 
   // Barriers and buffers go by the tile's number n in the block's life; `live`
   // counts its items that have tiles.
@@ -284,9 +291,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1);
       tc_fence_after();
       const bool seen = i < t.len;
-      store_row<T>(seen ? row_ptr<T>(a.out, t, item.h, i) : nullptr,
-                   seen && a.out_low.data ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr,
-                   tO + quad, D, ok ? 1.f / l : NAN);
+      const float inv = ok ? 1.f / l : NAN;
+      store_row<T>(seen ? row_ptr<T>(a.out, t, item.h, i) : nullptr, tO + quad, D, inv);
+      if (a.out_low.data)
+        store_row<T, true>(seen ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr, tO + quad, D,
+                           inv);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&sm.o_free));

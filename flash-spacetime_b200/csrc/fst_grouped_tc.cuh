@@ -176,18 +176,6 @@ __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// Two blocks of an SM that begin together would ask for the exponentials, and
-// for the tensor cores, at the same time all along: the one whose 256 columns
-// are the upper half of tensor memory starts `cycles`, half a tile, later
-// (forward of 8192 x 16 heads of 128: 510 -> 482 us).
-__device__ __forceinline__ void stagger(uint32_t tmem, uint32_t cycles) {
-  if (tmem & 256) {
-    const uint32_t start = (uint32_t)clock();
-    while ((uint32_t)clock() - start < cycles) {
-    }
-  }
-}
-
 // ---- pairs of fp32 values (one instruction for two lanes' worth) -------------
 
 using pair_t = unsigned long long;
@@ -304,27 +292,42 @@ __device__ __forceinline__ void zero_dead_rows(const FstRows& out, const RowTile
         make_uint4(0, 0, 0, 0);
 }
 
+// 16 channels, as one 32-byte store where the row lies on 32 bytes: a thread
+// writes whole sectors then, which the 32 rows of a warp's store touch one
+// each (two 16-byte stores pass every sector to L2 twice).
+__device__ __forceinline__ void store16(void* dst, const uint32_t (&w)[8]) {
+  if (((uintptr_t)dst & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    ((uint4*)dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    ((uint4*)dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
 // A thread's row of D accumulator columns, times f, rounded and stored (whole
-// warps; out may be null). What the rounding left over goes to `low`, if any.
-template <typename T>
-__device__ __forceinline__ void store_row(T* out, T* low, uint32_t acc, int D, float f) {
+// warps; out may be null). `Low`: what that rounding leaves over, instead.
+template <typename T, bool Low = false>
+__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f) {
   for (int d = 0; d < D; d += 32) {
     float o[32];
     tmem_ld32(o, acc + d);
     tmem_wait_ld();
     pin(o);
 #pragma unroll
-    for (int e = 0; e < 32; e += 8) {
+    for (int e = 0; e < 32; e += 16) {
       if (!out || d + e >= D) break;
-      uint32_t w[4], r[4];
+      uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const float x = o[e + 2 * i] * f, y = o[e + 2 * i + 1] * f;
         w[i] = Elem<T>::pack(x, y);
-        r[i] = Elem<T>::pack(x - Elem<T>::lo(w[i]), y - Elem<T>::hi(w[i]));
+        if (Low) w[i] = Elem<T>::pack(x - Elem<T>::lo(w[i]), y - Elem<T>::hi(w[i]));
       }
-      *(uint4*)(out + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
-      if (low) *(uint4*)(low + d + e) = make_uint4(r[0], r[1], r[2], r[3]);
+      if (d + e + 16 <= D)
+        store16(out + d + e, w);
+      else
+        *(uint4*)(out + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncwarp();  // tcgen05.ld takes the whole warp
   }

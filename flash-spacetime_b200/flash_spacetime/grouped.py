@@ -238,6 +238,10 @@ def flash_grouped_attention(
     events, rows, _, _ = _check_heads(q, k, v, layout)
     if isinstance(seqlens, Tensor) and seqlens.dim() == 1:
         _integers(seqlens, "seqlens")
+    for mask in (seqlens, key_padding_mask):
+        if isinstance(mask, Tensor) and mask.dim() == 2 and mask.shape != (events, rows):
+            raise ValueError(f"a padding mask must be [B, L] = [{events}, {rows}], got "
+                             f"{tuple(mask.shape)}")
     lens, _ = _padded_lengths(seqlens, key_padding_mask, events, rows, q.device, validate_mask,
                               None)
     lens = _integers(torch.as_tensor(lens), "seqlens")

@@ -285,3 +285,100 @@ def test_rotary_then_attention(dtype):
             # of one row has dq = dk = 0 up to the rounding of D.
             assert (a - b[0]).norm() <= tol * (b.norm() + g[at:at + n].double().norm())
         at += n
+
+
+def test_offsets_past_32_bits():
+    # 70 000 rows of 256 heads of 128: 2.3e9 elements. Two short events, one at
+    # either end; every other row is of no event.
+    total, heads, dim = 70000, 256, 128
+    q = torch.zeros(total, heads, dim, device="cuda", dtype=BF16)
+    k, v = (torch.randn(total, 1, dim, device="cuda", dtype=BF16) for _ in range(2))
+    rows = torch.cat((torch.arange(40), torch.arange(total - 150, total))).cuda()
+    q[rows] = torch.randn(190, heads, dim, device="cuda", dtype=BF16)
+    g = torch.ones_like(q)
+    cu = torch.tensor([0, 40, 40, 40], dtype=torch.int32, device="cuda")
+    late = torch.tensor([total - 150, total], dtype=torch.int32, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    for offsets, part, lens in ((cu, slice(0, 40), [40]), (late, slice(total - 150, total), [150])):
+        out = flash_grouped_attention_varlen(q, k, v, offsets)
+        got = (out.detach(),) + torch.autograd.grad(out, leaves, g)
+        small = [t[part].detach().clone().requires_grad_(True) for t in (q, k, v)]
+        ref = flash_grouped_attention_varlen(*small, _offsets(lens))
+        want = (ref.detach(),) + torch.autograd.grad(ref, small, g[part])
+        for a, b in zip(got, want):
+            assert torch.equal(a[part], b)
+            assert a.flatten().count_nonzero() == b.count_nonzero()
+
+
+def test_two_streams_at_once():
+    # Calls that overlap share nothing: each gives what it gives alone.
+    lens = [700, 129, 40]
+    cu = _offsets(lens)
+    sets = [[torch.randn(sum(lens), h, d, device="cuda", dtype=t) for h in (4, 2, 2, 4)]
+            for d, t in ((64, BF16), (128, FP16))]
+
+    def run(q, k, v, g):
+        q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+        out = flash_grouped_attention_varlen(q, k, v, cu)
+        return (out.detach(),) + torch.autograd.grad(out, (q, k, v), g)
+
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (s, t) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(s):
+                got[i].append(run(*t))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (FP16, 128), (FP32, 32)])
+def test_a_nan_row_stays_visible(dtype, dim):
+    # A NaN in row 5 of k reaches every row of its event that sees it, and no
+    # row of another event.
+    q, k, v = (torch.randn(300, 2, dim, device="cuda", dtype=dtype) for _ in range(3))
+    cu = _offsets([100, 200])
+    clean = flash_grouped_attention_varlen(q, k, v, cu, causal=False)
+    k[5] = float("nan")
+    out = flash_grouped_attention_varlen(q, k, v, cu, causal=False)
+    assert out[:100].isnan().all()
+    assert torch.equal(out[100:], clean[100:])
+
+
+def test_gradients_are_differentiable_once():
+    q, k, v = (torch.randn(20, 1, 32, device="cuda", requires_grad=True) for _ in range(3))
+    out = flash_grouped_attention_varlen(q, k, v, _offsets([20]))
+    (dq,) = torch.autograd.grad(out.sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), q)
+
+
+def test_arguments_on_the_gpu_are_checked():
+    q = torch.randn(2, 4, 9, 32, device="cuda", dtype=BF16)
+    k = torch.randn(2, 2, 9, 32, device="cuda", dtype=BF16)
+    bad = [
+        (dict(k=k.float()), "dtype"), (dict(k=k[:, :, :8], v=k[:, :, :8]), "rows"),
+        (dict(v=k[..., :16]), "rows"), (dict(k=k.cpu()), "CUDA"),
+        (dict(k=torch.cat((k, k[:, :1]), 1), v=torch.cat((k, k[:, :1]), 1)), "multiple"),
+        (dict(layout="packed"), "varlen"), (dict(layout="x"), "layout"),
+        (dict(seqlens=torch.tensor([1.0, 2.0])), "integers"), (dict(seqlens=[1, 2, 3]), "seqlens"),
+        (dict(seqlens=torch.zeros(2, 8, dtype=torch.bool)), "mask"),
+        (dict(seqlens=[1, 2], key_padding_mask=torch.zeros(2, 9, dtype=torch.bool)), "not both"),
+        (dict(q=torch.randn(2, 4, 9, 136, device="cuda"),
+              k=torch.randn(2, 4, 9, 136, device="cuda"),
+              v=torch.randn(2, 4, 9, 136, device="cuda")), "128"),
+        (dict(scale=float("nan")), "finite"),
+    ]
+    for change, text in bad:
+        args = dict(q=q, k=k, v=k)
+        args.update(change)
+        with pytest.raises(ValueError, match=text):
+            flash_grouped_attention(**args)
+    packed = [t.transpose(1, 2).flatten(0, 1) for t in (q, k, k)]
+    for cu in (torch.tensor([[0, 9]]), torch.tensor([0.0, 9.0]), torch.zeros(0, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            flash_grouped_attention_varlen(*packed, cu)

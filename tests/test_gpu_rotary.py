@@ -149,3 +149,51 @@ def test_graph_replay():
     fixed.copy_(x)
     graph.replay()
     assert torch.equal(out, flash_rotary_varlen(x, None, freqs, cu)[0])
+
+
+def test_offsets_past_32_bits():
+    # 70 000 rows of 256 heads of 128: 2.3e9 elements.
+    x = torch.zeros(70000, 256, 128, device="cuda", dtype=BF16)
+    x[-3:] = torch.randn(3, 256, 128, device="cuda", dtype=BF16)
+    freqs = rotary_frequencies(128)
+    pos = torch.arange(70000, device="cuda")
+    got, _ = flash_rotary_varlen(x, None, freqs, positions=pos)
+    _check(got[-3:], x[-3:], freqs, pos[-3:, None], False, 1.0)
+    assert got[:-3].count_nonzero() == 0
+
+
+def test_outputs_may_be_the_inputs():
+    # The C ABI allows it: every thread reads what it writes.
+    import ctypes
+    from flash_spacetime import _lib
+    x = torch.randn(33, 5, 64, device="cuda", dtype=BF16)
+    freqs = rotary_frequencies(48).cuda()
+    pos = torch.arange(33, device="cuda")
+    want, _ = flash_rotary_varlen(x, None, freqs, positions=pos)
+    a = _lib.FstRotaryArgs()
+    a.dtype, a.packed, a.heads, a.head_dim, a.pairs, a.positions_64 = _lib.FST_BF16, 1, 5, 64, 24, 1
+    a.magnitude, a.total_rows, a.freqs, a.positions = 1.0, 33, freqs.data_ptr(), pos.data_ptr()
+    a.q = a.q_out = _lib.FstRows(x.data_ptr(), 0, 64, 5 * 64)
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(_lib.load().fst_rotary(ctypes.byref(a), stream), "fst_rotary")
+    assert torch.equal(x, want)
+
+
+def test_arguments_on_the_gpu_are_checked():
+    q = torch.randn(2, 4, 9, 32, device="cuda")
+    k = torch.randn(2, 2, 9, 32, device="cuda")
+    freqs = rotary_frequencies(32)
+    bad = [
+        (dict(k=k.half()), "dtype"), (dict(k=k[:, :, :8]), "rows"), (dict(k=k[..., :16]), "rows"),
+        (dict(k=k.cpu()), "CUDA"), (dict(freqs=rotary_frequencies(34)), "freqs"),
+        (dict(freqs=freqs[None]), "freqs"), (dict(freqs=torch.arange(4)), "freqs"),
+        (dict(freqs=freqs.clone().requires_grad_(True)), "grad"),
+        (dict(positions=torch.zeros(9)), "integers"),
+        (dict(positions=torch.zeros(2, 8, dtype=torch.int64)), "positions"),
+        (dict(magnitude=float("inf")), "finite"), (dict(layout="packed"), "layout"),
+    ]
+    for change, text in bad:
+        args = dict(q=q, k=k, freqs=freqs)
+        args.update(change)
+        with pytest.raises(ValueError, match=text):
+            flash_rotary(**args)
