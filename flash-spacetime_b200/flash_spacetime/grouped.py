@@ -144,7 +144,7 @@ def _forward(q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str, scale: 
     out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     low = torch.empty_like(out) if keep_low and q.element_size() == 2 else None
     shape = (heads, rows) if layout == "packed" else (events, heads, rows)
-    lse = torch.empty(shape, dtype=torch.float32, device=q.device)
+    lse = q.new_empty(shape, dtype=torch.float32)
     args = _FORWARD.pack(
         *_problem(q, _shape(k, layout, "k")[2], layout, lens, scale, causal), *_rows(q, layout),
         *_rows(k, layout), *_rows(v, layout), *_rows(out, layout),
@@ -163,22 +163,32 @@ class _FlashGroupedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad_out: Tensor) -> Tuple[Optional[Tensor], ...]:  # type: ignore[override]
-        q, k, v, out, low, lse, lens = ctx.saved_tensors
-        layout = ctx.layout
-        dout = _in_place(grad_out)
-        dq, dk, dv = (torch.empty_like(t, memory_format=_CONTIGUOUS) for t in (q, k, v))
-        stats = torch.empty(2 * lse.numel(), dtype=torch.float32, device=q.device)
-        args = _BACKWARD.pack(
-            *_problem(q, _shape(k, layout, "k")[2], layout, lens, ctx.scale, ctx.causal),
-            *_rows(q, layout), *_rows(k, layout), *_rows(v, layout), *_rows(out, layout),
-            *(_NO_ROWS if low is None else _rows(low, layout)), *_rows(dout, layout),
-            *_rows(dq, layout), *_rows(dk, layout), *_rows(dv, layout), lse.data_ptr(), stats.data_ptr())
-        _call("fst_grouped_backward", args, q.device)
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
-                None, None, None, None)
+        return once(_backward)(ctx, grad_out)
+
+
+def once(backward: Callable[..., Any]) -> Callable[..., Any]:
+    """``backward``, refusing to be differentiated again. Only a backward pass
+    that builds a graph itself can be, and only it pays for the refusal."""
+    return once_differentiable(backward) if torch.is_grad_enabled() else backward
+
+
+def _backward(ctx: Any, grad_out: Tensor) -> Tuple[Optional[Tensor], ...]:
+    """One ``fst_grouped_backward`` call."""
+    q, k, v, out, low, lse, lens = ctx.saved_tensors
+    layout = ctx.layout
+    dout = _in_place(grad_out)
+    dq, dk, dv = (torch.empty_like(t, memory_format=_CONTIGUOUS) for t in (q, k, v))
+    stats = lse.new_empty(2 * lse.numel())
+    args = _BACKWARD.pack(
+        *_problem(q, _shape(k, layout, "k")[2], layout, lens, ctx.scale, ctx.causal),
+        *_rows(q, layout), *_rows(k, layout), *_rows(v, layout), *_rows(out, layout),
+        *(_NO_ROWS if low is None else _rows(low, layout)), *_rows(dout, layout),
+        *_rows(dq, layout), *_rows(dk, layout), *_rows(dv, layout), lse.data_ptr(), stats.data_ptr())
+    _call("fst_grouped_backward", args, q.device)
+    need = ctx.needs_input_grad
+    return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
+            None, None, None, None)
 
 
 def _check_heads(q: Tensor, k: Tensor, v: Tensor, layout: str) -> Sizes:

@@ -12,9 +12,8 @@ from typing import Any, Optional, Tuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
-from .grouped import _CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _integers, _rows, _shape
+from .grouped import _CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _integers, _rows, _shape, once
 from .ops import _DTYPES
 
 _ROTARY = struct.Struct("@11ifq3Q" + 4 * _ROWS)
@@ -61,18 +60,21 @@ class _FlashRotary(torch.autograd.Function):
         return _rotate(q, k, freqs, cu, positions, layout, interleaved, magnitude, False)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, gq: Optional[Tensor], gk: Optional[Tensor]):  # type: ignore[override]
-        freqs, cu, positions = ctx.saved_tensors
-        layout, interleaved, magnitude = ctx.how
-        gq = gq if ctx.needs_input_grad[0] else None
-        gk = gk if ctx.needs_input_grad[1] else None
-        dq = dk = None
-        if gq is not None:
-            dq, dk = _rotate(gq, gk, freqs, cu, positions, layout, interleaved, magnitude, True)
-        elif gk is not None:
-            dk, _ = _rotate(gk, None, freqs, cu, positions, layout, interleaved, magnitude, True)
-        return dq, dk, None, None, None, None, None, None
+        return once(_backward)(ctx, gq, gk)
+
+
+def _backward(ctx: Any, gq: Optional[Tensor], gk: Optional[Tensor]) -> Tuple[Any, ...]:
+    freqs, cu, positions = ctx.saved_tensors
+    layout, interleaved, magnitude = ctx.how
+    gq = gq if ctx.needs_input_grad[0] else None
+    gk = gk if ctx.needs_input_grad[1] else None
+    dq = dk = None
+    if gq is not None:
+        dq, dk = _rotate(gq, gk, freqs, cu, positions, layout, interleaved, magnitude, True)
+    elif gk is not None:
+        dk, _ = _rotate(gk, None, freqs, cu, positions, layout, interleaved, magnitude, True)
+    return dq, dk, None, None, None, None, None, None
 
 
 def _apply(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
