@@ -42,6 +42,21 @@ constexpr int kBM = 128;  // rows a block owns
 constexpr int threads_of(int W) { return W * 128 + 64; }
 constexpr int resident_of(int W) { return W == 1 ? 2 : 1; }
 
+// Events of so few rows take dS in two 16-bit parts, and one more product. With
+// two keys dS_1 = -dS_2, and its rounding goes into dq whole (1.6 times the
+// error of rounding dq itself); over more keys the roundings average out (1.4
+// times from 4 keys on, however many).
+constexpr int kFew = 32;
+template <typename T>
+__device__ __forceinline__ void store_rest(uint32_t dst, const float (&x)[32],
+                                           const uint32_t (&rounded)[16]) {
+  uint32_t w[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    w[e] = Elem<T>::pack(x[2 * e] - Elem<T>::lo(rounded[e]), x[2 * e + 1] - Elem<T>::hi(rounded[e]));
+  tmem_st16(dst, w);
+}
+
 // ---- dq ---------------------------------------------------------------------
 
 template <int Boxes, int W, int Stages>
@@ -126,6 +141,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const int n = uniform(tiles), last = uniform(end), dim = uniform(D);
     const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, q_mem = p_mem + kBN;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
+    const bool few = uniform(t.len) <= kFew;  // one tile then
     auto keys = [&](int it) { return min(kBN, last - it * kBN); };
     auto logits = [&](int it) {
       if (!mbar_wait(smem_addr(&sm.full[it % Stages]), (it / Stages) & 1)) return false;
@@ -153,6 +169,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       tc_fence_after();
       accumulate<kBN>(q_mem, p_mem, smem_addr(sm.k[it % Stages]), keys(it), acc_instr, it > 0,
                       leader);
+      if (few) accumulate<kBN>(q_mem, p_mem + 32, smem_addr(sm.k[0]), last, acc_instr, true, leader);
       tc_commit(smem_addr(&sm.empty[it % Stages]), leader);
       if (it + 1 < n) weights(it + 1);
     }
@@ -199,8 +216,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     }
     const pair_t scale2 = pair(c2, c2), lse2n = pair(-lse2, -lse2), delta2n = pair(-delta, -delta);
     // One tile. `Whole`: every row of the block sees all its keys.
-    auto tile = [&](auto whole, int it) {
-      constexpr bool Whole = decltype(whole)::value;
+    auto tile = [&](auto whole, auto is_few, int it) {
+      constexpr bool Whole = decltype(whole)::value, Few = decltype(is_few)::value;
       const int j0 = it * kBN + w * 64, nk = end - j0;
       if (!mbar_wait(smem_addr(&sm.s_full), it & 1)) return false;
       tc_fence_after();
@@ -247,6 +264,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = Elem<T>::pack(dp[2 * e], dp[2 * e + 1]);
         tmem_st16(tP + c * 16, x);
+        if (Few && c == 0) store_rest<T>(tP + 32, dp, x);
       }
       const int all = min(kBN, end - it * kBN);
       if (!Whole && (all & 15))  // dS is 0 there, and must not meet another event's NaN
@@ -259,8 +277,9 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     };
     const int whole = min(tiles, (p.causal ? min(t.len, t.i0 + 1) : t.len) / kBN);
     int it = 0;
-    for (; it < whole && ok; ++it) ok = tile(std::true_type(), it);
-    for (; it < tiles && ok; ++it) ok = tile(std::false_type(), it);
+    for (; it < whole && ok; ++it) ok = tile(std::true_type(), std::false_type(), it);
+    if (t.len <= kFew) ok = tile(std::false_type(), std::true_type(), it++);
+    for (; it < tiles && ok; ++it) ok = tile(std::false_type(), std::false_type(), it);
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
     // The groups share the columns of the result.
@@ -377,6 +396,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, v_mem = p_mem + kBN,
                    k_mem = v_mem + kAcc;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
+    const bool few = uniform(t.len) <= kFew;  // one tile a head then
     // S^T over P^T and dP^T over dS^T: MMAs complete in order, so the products
     // that read those are done.
     auto logits = [&](int it, int q_rows) {
@@ -407,6 +427,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       if (!ok) break;
       tc_fence_after();
       accumulate<kBN>(k_mem, p_mem, smem_addr(sm.q[s]), q_rows, acc_instr, it > 0, leader);
+      if (few)
+        accumulate<kBN>(k_mem, p_mem + 32, smem_addr(sm.q[s]), q_rows, acc_instr, true, leader);
       tc_commit(smem_addr(&sm.empty[s]), leader);
       if (it + 1 < n) weights(it + 1, next_rows);
       q_rows = next_rows;
@@ -504,6 +526,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = Elem<T>::pack(dp[2 * e], dp[2 * e + 1]);
         tmem_st16(tP + c * 16, y);
+        if (c == 0 && t.len <= kFew) store_rest<T>(tP + 32, dp, y);
       }
       tmem_wait_st();
       tc_fence_before();

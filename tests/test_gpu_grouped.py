@@ -64,6 +64,29 @@ def test_packed_lengths(dim, causal, lens):
     _packed(lens, 2, 2, dim, BF16, causal, seed=len(lens))
 
 
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (FP16, 32), (BF16, 128), (BF16, 24)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_very_short_events(dtype, dim, causal):
+    # Up to 32 rows dS is kept in two 16-bit parts (its rest is below 2^-16 of
+    # it), so dq and dk are off by their own rounding, u |.|, and terms of the
+    # order of fp32 (the bound's, with the rounding of P and dS taken out).
+    lens = [2, 1, 3, 32, 7, 2, 31]
+    events = gc.make_case(lens, 4, 2, dim, dtype, causal, seed=21)
+    q, k, v, g = (gc.pack(events, x).cuda() for x in "qkvg")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = flash_grouped_attention_varlen(*leaves, _offsets(lens), causal=causal)
+    dq, dk, _ = torch.autograd.grad(out, leaves, g)
+    u, at = gc.HALF_STEP[dtype], 0
+    for n, ev in zip(lens, events):
+        for name, t, other in (("dq", dq, "k"), ("dk", dk, "q")):
+            err = (t[at:at + n].transpose(0, 1).double().cpu() - ev[name]).abs()
+            # dS <= |dP| + |D| <= 2 max |g| |v|; 2^-14 covers both parts' rest.
+            size = 2 * ev["g"].double().norm(dim=-1).max() * ev["v"].double().norm(dim=-1).max()
+            loose = 2.0**-14 * dim**-0.5 * size * ev[other].double().abs().max() * n * 2
+            assert (err <= u * ev[name].abs() + loose).all(), (name, n)
+        at += n
+
+
 @pytest.mark.parametrize("heads, kv_heads", [(1, 1), (5, 1), (6, 3), (16, 2), (3, 3)])
 @pytest.mark.parametrize("dim, dtype", [(32, BF16), (64, FP16), (128, BF16), (32, FP32)])
 def test_head_groups(heads, kv_heads, dim, dtype):
