@@ -44,10 +44,9 @@ __device__ __forceinline__ int entry_row(const FstGroupedProblem& p, int e) {
   return clamp_row(__ldg(p.cu_seqlens + e), p.total_rows);
 }
 
-// Entry `id` of the list (called by whole warps). Causal blocks of an event
-// come last rows first (`heavy_last` false) or first rows first, whichever
-// puts the ones with most keys or queries at the front. Returns false when
-// the position is empty.
+// Block `id` of the list (called by whole warps). `reverse`: an event's live
+// blocks last rows first, which puts the causal ones with most keys at the
+// front. Returns false when the position is empty.
 template <int BM>
 __device__ __forceinline__ bool find_tile(const FstGroupedProblem& p, int id, bool reverse,
                                           RowTile& t) {
@@ -87,9 +86,8 @@ __device__ __forceinline__ bool find_tile(const FstGroupedProblem& p, int id, bo
   }
   live = (t.len + BM - 1) / BM;
   if (reverse && tile < live) tile = live - 1 - tile;
-  // A position behind the entry's last block is empty (and tile * BM stays
-  // far below 2^31: tile <= list_blocks <= 2^31 / BM + B + 2 only for BM >= 64
-  // and rows < 2^31, so compare before multiplying).
+  // A position behind the entry's last block is empty (compared before tile is
+  // multiplied: positions of other entries' blocks may lie far behind).
   if (tile >= (t.lim + BM - 1) / BM) return false;
   t.i0 = tile * BM;
   return true;

@@ -26,6 +26,11 @@
 // Above, dV and dK (or dQ) need twice the columns; two groups and one block,
 // whose products are 128 wide: a product of two shared-memory operands reads
 // 4 KB of A per 16 channels whatever its width, which bounds 64 wide ones.
+//
+// Measured, bf16, 8192 rows, 16 heads, not causal: rows 728 us, columns 809 us
+// at Dh = 128; 423 and 661 us at 64; 410 and 607 us at 32. At 128 the tensor
+// cores are busy half the time, at 64 the exponentials' unit; what remains is
+// the chain of a tile's steps.
 
 #include <cuda_runtime.h>
 

@@ -1,14 +1,22 @@
 // Grouped-head attention, forward, on the tensor cores (16-bit inputs).
 //
-// One block owns 128 query rows of one event and head and walks the event's
-// keys in tiles of kBN, twice resident on each SM so that one block's softmax
-// runs beside the other's products:
-//   warp 4   brings Q once and the K and V tiles by TMA;
+// An item is 128 query rows of one event and head; its keys come in tiles of
+// kBN. A block works through many items (Feed), two blocks to an SM, so that
+// one's softmax runs beside the other's products:
+//   warp 4   feeds: looks items up, brings Q and the K and V tiles by TMA;
 //   warp 5   issues S = Q K^T into tensor memory, one tile ahead (two S
 //            buffers), and O += P V from it;
 //   warps 0-3, one thread a query row: reads S, keeps the running maximum and
 //            sum, writes P back over S as 16-bit values (the A operand of the
 //            second product), rescales O when the maximum has grown.
+//
+// Measured, bf16, 8192 rows, 16 heads, not causal: 507 us at Dh = 128 (1080
+// TFLOP/s; the 64-wide Q K^T reads 4 KB of Q for every 2 KB of K, and O and
+// two S fill the 256 columns), 390 us at 64 and 382 us at 32, where the 2.7e12
+// exponentials a second are 60 % of the unit's 16 a cycle and SM: the rest is
+// the chain from one tile's S to its P (load 200 cycles, maximum 100, vote 90,
+// exponentials 770, stores and barriers 200). Tiles whose keys all rows see
+// run without masks (16384 causal of 64: 540 -> 470 us).
 //
 // Softmax in the base-2 domain: p = 2^(c s - c m), c = |scale| log2(e) (the
 // sign of the scale is the product's own negate bit). O and l are rescaled
