@@ -40,6 +40,7 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kBN = 64;
 constexpr int kThreads = 192;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kGrow = 8.f;  // log2 of the growth that forces a rescale
 
 template <int Boxes, int Stages>
@@ -112,8 +113,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       item.kh = at.kh;
       if (find_tile<kBM>(p, at.id, p.causal, item.t)) {
         const RowTile& t = item.t;
-        const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
-        item.tiles = t.i0 < t.len ? (end + kBN - 1) / kBN : 0;
+        item.end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
+        item.tiles = t.i0 < t.len ? (item.end + kBN - 1) / kBN : 0;
+        item.whole = min(item.tiles, (p.causal ? min(t.len, t.i0 + 1) : t.len) / kBN);
+        item.dead = min(t.i0 + kBM, t.lim) > t.len;
+        item.out_at = row_ptr<T>(a.out, t, item.h, t.i0) - (T*)a.out.data;
+        item.stat_at = stat_at(p, t, p.heads, item.h, t.i0);
         ok = feed_put(sm.feed, c++, item, most, lane);
         if (item.tiles && ok) {
           if (lane == 0) {
@@ -161,8 +166,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int c = 0, n = 0, live = 0; ok && feed_take(sm.feed, c, item, lane); ++c) {
       const int tiles = uniform(item.tiles);
       if (!tiles) continue;
-      const int last =
-          uniform(p.causal ? min(item.t.len, item.t.i0 + kBM) : item.t.len);
+      const int last = uniform(item.end);
       auto keys = [&](int it) { return min(kBN, last - it * kBN); };
       // S of a tile. Its buffer may be overwritten: MMAs complete in order,
       // so the product that read P from it two tiles ago is done by then.
@@ -202,9 +206,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     Item item;
     for (int c = 0, n = 0; ok && feed_take(sm.feed, c, item, lane); ++c) {
       const RowTile& t = item.t;
-      zero_dead_rows<T, kBM>(a.out, t, item.h, D, 128);
+      if (item.dead) zero_dead_rows<T, kBM>(a.out, t, item.h, D, 128);
       if (!item.tiles) continue;
-      const int end = p.causal ? min(t.len, t.i0 + kBM) : t.len;
+      const int end = item.end;
       const int i = t.i0 + warp * 32 + lane;
       float m = -INFINITY, l = 0.f;
       // One tile. `Whole`: every row of the block sees all its keys.
@@ -292,23 +296,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         ++n;
         return true;
       };
-      const int whole = min(item.tiles, (p.causal ? min(t.len, t.i0 + 1) : t.len) / kBN);
       int it = 0;
-      for (; it < whole && ok; ++it) ok = tile(std::true_type(), it);
+      for (; it < item.whole && ok; ++it) ok = tile(std::true_type(), it);
       for (; it < item.tiles && ok; ++it) ok = tile(std::false_type(), it);
+      // All but the output itself, while the last product runs.
+      const bool seen = i < t.len;
+      const int row = i - t.i0;
+      const float inv = ok ? 1.f / l : NAN;
+      if (seen) a.lse[item.stat_at + row] = ok ? (m * c2 + log2f(l)) * kLn2 : NAN;
+      T* out = seen ? (T*)a.out.data + item.out_at + row * a.out.row_stride : nullptr;
       if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1);
       tc_fence_after();
-      const bool seen = i < t.len;
-      const float inv = ok ? 1.f / l : NAN;
-      store_row<T>(seen ? row_ptr<T>(a.out, t, item.h, i) : nullptr, tO + quad, D, inv);
+      store_row<T>(out, tO + quad, D, ok ? inv : NAN);
       if (a.out_low.data)
         store_row<T, true>(seen ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr, tO + quad, D,
                            inv);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&sm.o_free));
-      if (seen)
-        a.lse[stat_at(p, t, p.heads, item.h, i)] = ok ? (m * c2 + log2f(l)) / kLog2e : NAN;
     }
     tc_fence_before();
   }

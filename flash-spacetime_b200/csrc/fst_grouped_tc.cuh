@@ -359,6 +359,10 @@ struct Item {
   RowTile t;
   int h, kh;
   int tiles;  // of the other side; 0: only rows of no event; below 0: the end
+  int whole;  // the first of them, whose keys all rows see
+  int end;    // keys the block's rows see
+  bool dead;  // some rows belong to no event
+  int64_t out_at, stat_at;  // elements: the output's row i0, its statistics
 };
 
 struct Feed {
