@@ -55,7 +55,8 @@ struct FwdSmem {
   uint32_t tmem;
 };
 
-template <typename T, int Boxes, int Stages>
+// Low: what rounding the output leaves over is kept too (training).
+template <typename T, int Boxes, int Stages, bool Low>
 __global__ void __launch_bounds__(kThreads, 2)
     fwd_kernel(const __grid_constant__ TileMaps maps, const FstGroupedForwardArgs a, int blocks) {
   using Smem = FwdSmem<Boxes, Stages>;
@@ -307,10 +308,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       T* out = seen ? (T*)a.out.data + item.out_at + row * a.out.row_stride : nullptr;
       if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1);
       tc_fence_after();
-      store_row<T>(out, tO + quad, D, ok ? inv : NAN);
-      if (a.out_low.data)
-        store_row<T, true>(seen ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr, tO + quad, D,
-                           inv);
+      const float f = ok ? inv : NAN;
+      T* low = Low && seen ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr;
+      if (Low && Boxes == 1) {
+        store_row<T, false, true>(out, tO + quad, D, f, low);
+      } else {
+        // Two passes over a wide row: one would cost the main loop registers.
+        store_row<T>(out, tO + quad, D, f);
+        if (Low) store_row<T, true>(low, tO + quad, D, f);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&sm.o_free));
@@ -322,11 +328,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 5) tmem_free<kCols>(tmem);
 }
 
-template <typename T, int Boxes, int Stages>
+template <typename T, int Boxes, int Stages, bool Low>
 int launch(const FstGroupedForwardArgs& a, cudaStream_t st) {
   const FstGroupedProblem& p = a.prob;
   static std::atomic<uint64_t> done{0};
-  const auto kernel = fwd_kernel<T, Boxes, Stages>;
+  const auto kernel = fwd_kernel<T, Boxes, Stages, Low>;
   const int bytes = (int)sizeof(FwdSmem<Boxes, Stages>) + 1024;
   const int e = allow_dynamic_smem((const void*)kernel, bytes, done);
   if (e) return api_fail(FST_ERR_CUDA, "shared memory: %s", cudaGetErrorString((cudaError_t)e));
@@ -345,8 +351,9 @@ int launch(const FstGroupedForwardArgs& a, cudaStream_t st) {
 
 template <typename T>
 int launch_t(const FstGroupedForwardArgs& a, cudaStream_t st) {
-  if (a.prob.head_dim <= 64) return launch<T, 1, 3>(a, st);
-  return launch<T, 2, 2>(a, st);
+  const bool low = a.out_low.data != nullptr;
+  if (a.prob.head_dim <= 64) return low ? launch<T, 1, 3, true>(a, st) : launch<T, 1, 3, false>(a, st);
+  return low ? launch<T, 2, 2, true>(a, st) : launch<T, 2, 2, false>(a, st);
 }
 
 }  // namespace

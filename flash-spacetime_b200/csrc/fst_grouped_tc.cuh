@@ -306,9 +306,11 @@ __device__ __forceinline__ void store16(void* dst, const uint32_t (&w)[8]) {
   }
 }
 // A thread's row of D accumulator columns, times f, rounded and stored (whole
-// warps; out may be null). `Low`: what that rounding leaves over, instead.
-template <typename T, bool Low = false>
-__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f) {
+// warps; out may be null). `Low`: what that rounding leaves over, instead;
+// `Both`: that too, to `low` (may be null), in one pass over the accumulator.
+template <typename T, bool Low = false, bool Both = false>
+__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f,
+                                          T* low = nullptr) {
   for (int d = 0; d < D; d += 32) {
     float o[32];
     tmem_ld32(o, acc + d);
@@ -317,17 +319,21 @@ __device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f) 
 #pragma unroll
     for (int e = 0; e < 32; e += 16) {
       if (!out || d + e >= D) break;
-      uint32_t w[8];
+      auto put = [&](T* dst, const uint32_t (&w)[8]) {
+        if (d + e + 16 <= D)
+          store16(dst + d + e, w);
+        else
+          *(uint4*)(dst + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+      };
+      uint32_t w[8], r[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = o[e + 2 * i] * f, y = o[e + 2 * i + 1] * f;
         w[i] = Elem<T>::pack(x, y);
-        if (Low) w[i] = Elem<T>::pack(x - Elem<T>::lo(w[i]), y - Elem<T>::hi(w[i]));
+        if (Low || Both) r[i] = Elem<T>::pack(x - Elem<T>::lo(w[i]), y - Elem<T>::hi(w[i]));
       }
-      if (d + e + 16 <= D)
-        store16(out + d + e, w);
-      else
-        *(uint4*)(out + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+      put(out, Low ? r : w);
+      if (Both && low) put(low, r);
     }
     __syncwarp();  // tcgen05.ld takes the whole warp
   }
