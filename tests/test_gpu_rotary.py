@@ -197,3 +197,27 @@ def test_arguments_on_the_gpu_are_checked():
         args.update(change)
         with pytest.raises(ValueError, match=text):
             flash_rotary(**args)
+
+
+def test_gradient_of_q_alone():
+    q = torch.randn(30, 2, 32, device="cuda", requires_grad=True)
+    freqs, cu = rotary_frequencies(32), torch.tensor([0, 12, 30], device="cuda")
+    out, none = flash_rotary_varlen(q, None, freqs, cu, magnitude=0.5)
+    g = torch.randn_like(q)
+    (dq,) = torch.autograd.grad(out, q, g)
+    assert none is None
+    _check(dq, g, -freqs, _event_positions([12, 18])[:, None], False, 0.5)
+
+
+def test_gradient_against_differences():
+    # The op is linear: its difference along d is its value at d, up to the
+    # fp32 rounding of 240 products of order 1.
+    q, d, w = (torch.randn(10, 1, 24, device="cuda") for _ in range(3))
+    q.requires_grad_(True)
+    freqs, cu = rotary_frequencies(24), torch.tensor([0, 4, 10], device="cuda")
+    (dq,) = torch.autograd.grad(flash_rotary_varlen(q, None, freqs, cu)[0], q, w)
+    with torch.no_grad():
+        far = (flash_rotary_varlen(q + d, None, freqs, cu)[0].double()
+               - flash_rotary_varlen(q, None, freqs, cu)[0].double())
+    want = (far * w.double()).sum()
+    assert abs((dq.double() * d.double()).sum() - want) <= 2.0**-20 * 240 * 16
