@@ -453,8 +453,11 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       const int lo = p.causal ? j - qw : 0;  // columns lo <= c < nq see key j
       const float* ls = &sm.lse2n[s][w * 64];
       const float* de = &sm.deltan[s][w * 64];
-      ok = mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1) &&
-           mbar_wait(smem_addr(&sm.s_full), it & 1);
+      ok = mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1);
+      ulonglong2 ahead[8];  // the first half's statistics, read before they are needed
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ahead[e] = *(const ulonglong2*)(ls + e * 4);
+      ok = ok && mbar_wait(smem_addr(&sm.s_full), it & 1);
       if (!ok) break;
       tc_fence_after();
       float x[2][32];
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         pin(x[c]);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          const ulonglong2 l4 = *(const ulonglong2*)(ls + c * 32 + e);
+          const ulonglong2 l4 = c ? *(const ulonglong2*)(ls + c * 32 + e) : ahead[e / 4];
 #pragma unroll
           for (int f = 0; f < 4; f += 2) {
             const float2 y =
@@ -499,6 +502,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&sm.p_ready));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ahead[e] = *(const ulonglong2*)(de + e * 4);
       ok = mbar_wait(smem_addr(&sm.dp_full), it & 1);
       if (!ok) break;
       tc_fence_after();
@@ -511,7 +516,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         pin(dp);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          const ulonglong2 d4 = *(const ulonglong2*)(de + c * 32 + e);
+          const ulonglong2 d4 = c ? *(const ulonglong2*)(de + c * 32 + e) : ahead[e / 4];
 #pragma unroll
           for (int f = 0; f < 4; f += 2) {
             const float2 y = split(mul2(pair(x[c][e + f], x[c][e + f + 1]),
