@@ -27,8 +27,8 @@
 // whose products are 128 wide: a product of two shared-memory operands reads
 // 4 KB of A per 16 channels whatever its width, which bounds 64 wide ones.
 //
-// Measured, bf16, 8192 rows, 16 heads, not causal: rows 728 us, columns 809 us
-// at Dh = 128; 423 and 661 us at 64; 410 and 607 us at 32. At 128 the tensor
+// Measured, bf16, 8192 rows, 16 heads, not causal: rows 728 us, columns 810 us
+// at Dh = 128; 423 and 637 us at 64; 410 and 592 us at 32. At 128 the tensor
 // cores are busy half the time, at 64 the exponentials' unit; what remains is
 // the chain of a tile's steps.
 
@@ -494,7 +494,9 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       }
       if (all & 15) {
         // Rows up to the next multiple of 16 have P = dS = 0, and must not meet
-        // another event's NaN. (A dP^T still reading dO there is masked.)
+        // another event's NaN. dP^T has to have read dO by then.
+        ok = mbar_wait(smem_addr(&sm.dp_full), it & 1);
+        if (!ok) break;
         zero_tile_rows<Boxes, kBN>(sm.q[s], all, (all + 15) & ~15, threadIdx.x, W * 128);
         zero_tile_rows<Boxes, kBN>(sm.g[s], all, (all + 15) & ~15, threadIdx.x, W * 128);
       }

@@ -20,7 +20,10 @@ Conventions:
   unrounded output: rows of few keys would otherwise carry its rounding into
   dq and dk;
 * inputs are read in place whatever their strides, as long as the channels of
-  a head are adjacent: slices of a fused projection need no copy.
+  a head are adjacent: slices of a fused projection need no copy;
+* forward and backward may be captured into CUDA graphs (lengths on the device;
+  a list is copied, which a capture refuses). PyTorch's own rule holds for
+  ``.backward()`` in a capture: no eager graph of the same leaves may be alive.
 """
 
 import struct
