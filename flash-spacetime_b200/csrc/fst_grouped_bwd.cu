@@ -244,8 +244,11 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       }
       if (!mbar_wait(smem_addr(&sm.dp_full), it & 1)) return false;
       tc_fence_after();
-      // Keys below lim are seen; the warp's first row sees fewest.
-      const int lim = (p.causal ? min(i + 1, t.len) : t.len) - j0;
+      // Keys below lim are seen; the warp's first row sees fewest. A row that
+      // sees one key has P = 1 and dP = D, so its dS is 0: formed from two
+      // sums of different order it would be their rounding.
+      const int keys = p.causal ? min(i + 1, t.len) : t.len;
+      const int lim = (keys > 1 ? keys : 0) - j0;
       const int fewest = Whole ? 64 : uniform(lim);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -451,6 +454,9 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       const int qw = q0 + w * 64, nq = t.len - qw;  // this group's columns
       const bool edge = nq < 64 || (p.causal && qw < t.i0 + kBM - 1);
       const int lo = p.causal ? j - qw : 0;  // columns lo <= c < nq see key j
+      // Row 0 of a causal event, and the row of an event of one, see one key:
+      // dS is 0 (see the row kernel).
+      const int ds_lo = p.causal ? max(lo, 1 - qw) : t.len > 1 ? 0 : 1;
       const float* ls = &sm.lse2n[s][w * 64];
       const float* de = &sm.deltan[s][w * 64];
       ok = mbar_wait(smem_addr(&sm.full[s]), (it / Stages) & 1);
@@ -531,7 +537,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int col = c * 32 + e;
-            dp[e] = col >= lo && col < nq ? dp[e] : 0.f;
+            dp[e] = col >= ds_lo && col < nq ? dp[e] : 0.f;
           }
         }
         uint32_t y[16];

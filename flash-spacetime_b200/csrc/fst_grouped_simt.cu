@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(FstGroupedBackwardArgs a) 
       const int last = p.causal ? min(i + 1, t.len) : t.len;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const bool seen = j0 + tx + 16 * c < last;
+        // A row that sees one key has P = 1 and dP = D: dS is 0, not the
+        // rounding of two sums of different order.
+        const bool seen = j0 + tx + 16 * c < last && last > 1;
         const float pr = exp2f(s[r][c] * c2 - lse2[r]);
         P[(4 * ty + r) * kPS + tx + 16 * c] = seen ? pr * (dp[r][c] - delta[r]) : 0.f;
       }
@@ -312,7 +314,8 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(FstGroupedBackwardArgs a)
           const bool seen = i < t.len && (!p.causal || t.i0 + 4 * ty + r <= i);
           const float pr = seen ? exp2f(s[r][c] * c2 - lse2[col]) : 0.f;
           P[(4 * ty + r) * kPS + col] = pr;
-          S[(4 * ty + r) * kPS + col] = seen ? pr * (dp[r][c] - delta[col]) : 0.f;
+          const bool several = p.causal ? i > 0 : t.len > 1;  // row i sees more than one key
+          S[(4 * ty + r) * kPS + col] = seen && several ? pr * (dp[r][c] - delta[col]) : 0.f;
         }
       __syncwarp();
       accumulate<DM>(P, G, ty, tx, dv);
