@@ -31,6 +31,7 @@ from typing import Any, Callable, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -176,6 +177,20 @@ def once(backward: Callable[..., Any]) -> Callable[..., Any]:
     return once_differentiable(backward) if torch.is_grad_enabled() else backward
 
 
+def seen_by_autograd(*tensors: Optional[Tensor]) -> bool:
+    """Whether a call must go through its ``autograd.Function``.
+
+    For a gradient, and wherever something else follows the call and would not
+    see a bare launch: a trace would record the empty output alone, and
+    forward-mode derivatives or ``torch.func`` transforms would be dropped
+    where the Function refuses them. Other calls launch directly.
+    """
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+            or torch._C._functorch.peek_interpreter_stack() is not None)
+
+
 def _backward(ctx: Any, grad_out: Tensor) -> Tuple[Optional[Tensor], ...]:
     """One ``fst_grouped_backward`` call."""
     q, k, v, out, low, lse, lens = ctx.saved_tensors
@@ -216,7 +231,7 @@ def _apply(q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str, scale: Op
            causal: bool) -> Tensor:
     args = (q, k, v, lens, layout, float(q.shape[-1]**-0.5 if scale is None else scale),
             bool(causal))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if seen_by_autograd(q, k, v):
         return _FlashGroupedAttention.apply(*args)
     return _forward(*args)[0]
 

@@ -13,7 +13,8 @@ from typing import Any, Optional, Tuple
 import torch
 from torch import Tensor
 
-from .grouped import _CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _integers, _rows, _shape, once
+from .grouped import (_CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _integers, _rows, _shape,
+                      once, seen_by_autograd)
 from .ops import _DTYPES
 
 _ROTARY = struct.Struct("@11ifq3Q" + 4 * _ROWS)
@@ -110,7 +111,7 @@ def _apply(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
             positions = positions.to(torch.int32)
         positions = positions.to(q.device).contiguous()
     args = (q, k, freqs, cu, positions, layout, bool(interleaved), float(magnitude))
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if seen_by_autograd(q, k):
         return _FlashRotary.apply(*args)
     return _rotate(*args, False)
 
