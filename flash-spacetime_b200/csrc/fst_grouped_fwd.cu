@@ -24,7 +24,12 @@
 // p <= 2^8 then, exact in effect because the same m divides out at the end.
 //
 // P is rounded to the input type for the second product (u of its type, the
-// one rounding besides the output's); l sums the unrounded fp32 values.
+// one rounding besides the output's). O is divided by the sum of the rounded
+// values, so the weights that made it sum to 1 and a common offset of v passes
+// through unharmed: the backward takes D = dO . O from it, and an offset's
+// share of an error there would not cancel against dP (dq of three keys with
+// v of mean 8: error 23 times that of one rounding, now 1.1). lse, from which
+// the backward forms P anew, is that of the unrounded fp32 sum.
 
 #include <cuda_runtime.h>
 
@@ -48,6 +53,7 @@ struct FwdSmem {
   alignas(1024) char q[Boxes * kBM * 128];
   alignas(1024) char k[Stages][Boxes * kBN * 128];
   alignas(1024) char v[Stages][Boxes * kBN * 128];
+  alignas(1024) uint4 ones[Boxes == 1 ? 16 * 8 : 1];  // 16 rows of 64 channels of 1
   Feed feed;
   uint64_t q_full, q_empty, o_free;
   uint64_t k_full[Stages], k_empty[Stages], v_full[Stages], v_empty[Stages];
@@ -62,7 +68,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   using Smem = FwdSmem<Boxes, Stages>;
   extern __shared__ char raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kCols = 256;  // two S buffers (P over them) of kBN = 64, O from 128
+  // Two S buffers (P over them) of kBN = 64, O from 128; up to Dh = 64 the sum
+  // of the rounded P from 192: a product with 16 columns of ones, which the
+  // tensor cores have time for (16384 causal of 64: 472 -> 478 us; summed by
+  // the softmax warps, three more instructions a pair, 520). Above, O takes all
+  // columns, and those warps sum (8192 x 16 of 128: 489 -> 496 us).
+  constexpr int kCols = 256;
+  constexpr bool kOnes = Boxes == 1;
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int D = p.head_dim;
@@ -86,6 +98,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     prefetch_map(&maps.q);
     prefetch_map(&maps.k);
     prefetch_map(&maps.v);
+  }
+  if (kOnes && threadIdx.x < 128) {
+    const uint32_t one = Elem<T>::pack(1.f, 1.f);
+    sm.ones[threadIdx.x] = make_uint4(one, one, one, one);
+    fence_proxy_async();
   }
   if (warp == 5) tmem_alloc<kCols>(smem_addr(&sm.tmem));
   tc_fence_before();
@@ -192,6 +209,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         tc_fence_after();
         accumulate<kBN>(o_mem, s_mem + g % 2 * kBN, smem_addr(sm.v[s]), keys(it), o_instr, it > 0,
                         leader);
+        if (kOnes)
+          accumulate<kBN, 0>(o_mem + 64, s_mem + g % 2 * kBN, smem_addr(sm.ones), keys(it),
+                             instruction<T>(16, true, false), it > 0, leader);
         tc_commit(smem_addr(&sm.pv_done[g % 2]), leader);
         tc_commit(smem_addr(&sm.v_empty[s]), leader);
         if (it + 2 < tiles) ok = logits(it + 2);
@@ -211,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!item.tiles) continue;
       const int end = item.end;
       const int i = t.i0 + warp * 32 + lane;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, l_used = 0.f;  // l_used: of the rounded P, if kOnes is not
       // One tile. `Whole`: every row of the block sees all its keys.
       auto tile = [&](auto whole, int it) {
         constexpr bool Whole = decltype(whole)::value;
@@ -255,16 +275,18 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (grow) {
               m = mx;
               l *= keep;
+              l_used *= keep;
             }
             if (!mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1)) return false;
             tc_fence_after();
 #pragma unroll 1
             for (int d = 0; d < D; d += 16) tmem_scale16(tO + quad + d, keep);
+            if (kOnes) tmem_scale16(tO + quad + 64, keep);
           }
         }
         const float off = m == -INFINITY ? 0.f : m * c2;
         const pair_t off2 = pair(-off, -off);
-        pair_t sums = pair(0.f, 0.f);
+        pair_t sums = pair(0.f, 0.f), used = sums;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (!Whole && c * 32 >= nk) continue;
@@ -275,11 +297,14 @@ __global__ void __launch_bounds__(kThreads, 2)
             x = make_float2(ex2(x.x), ex2(x.y));
             sums = add2(sums, pair(x.x, x.y));
             w[e / 2] = Elem<T>::pack(x.x, x.y);
+            if (!kOnes) used = add2(used, pair(Elem<T>::lo(w[e / 2]), Elem<T>::hi(w[e / 2])));
           }
           tmem_st16(tSt + c * 16, w);
         }
         const float2 halves = split(sums);
         l += halves.x + halves.y;
+        const float2 used_halves = split(used);
+        l_used += used_halves.x + used_halves.y;
         if (!Whole && (nk & 15)) {
           // Keys up to the next multiple of 16 have p = 0, but what V holds
           // there (another event's rows) must not be able to make 0 * NaN.
@@ -303,12 +328,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       // All but the output itself, while the last product runs.
       const bool seen = i < t.len;
       const int row = i - t.i0;
-      const float inv = ok ? 1.f / l : NAN;
       if (seen) a.lse[item.stat_at + row] = ok ? (m * c2 + log2f(l)) * kLn2 : NAN;
       T* out = seen ? (T*)a.out.data + item.out_at + row * a.out.row_stride : nullptr;
       if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1);
       tc_fence_after();
-      const float f = ok ? inv : NAN;
+      if (kOnes) l_used = tmem_ld1(tO + quad + 64);
+      const float f = ok ? 1.f / l_used : NAN;
       T* low = Low && seen ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr;
       if (Low && Boxes == 1) {
         store_row<T, false, true>(out, tO + quad, D, f, low);

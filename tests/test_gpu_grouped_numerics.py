@@ -78,3 +78,79 @@ def test_row_0_of_a_causal_event_has_no_gradient_of_q_and_k(dtype, dim):
     dq, dk, dv = torch.autograd.grad(out, leaves, only)
     assert dq.count_nonzero() == 0 and dk.count_nonzero() == 0
     assert dv[first].count_nonzero() > 0
+
+
+# Errors against float64 in units of what one rounding of the exact result
+# leaves. Limits are those of a float64 model of the documented roundings (P,
+# dS and the results), given with each, and a margin.
+
+
+def _definition(q, k, v, g, causal, scale):
+    """float64 out, dq, dk, dv of events ``[E, heads, n, D]``."""
+    q, k, v, g = (t.detach().double() for t in (q, k, v, g))
+    group = q.shape[1] // k.shape[1]
+    q, g = (t.unflatten(1, (-1, group)) for t in (q, g))
+    k, v = k[:, :, None], v[:, :, None]
+    s = scale * (q @ k.transpose(-1, -2))
+    if causal:
+        s = s + torch.full(s.shape[-2:], float("-inf"), dtype=s.dtype, device=s.device).triu(1)
+    p = s.softmax(-1)
+    dp = g @ v.transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    return {"out": (p @ v).flatten(1, 2), "dq": scale * (ds @ k).flatten(1, 2),
+            "dk": scale * (ds.transpose(-1, -2) @ q).sum(2),
+            "dv": (p.transpose(-1, -2) @ g).sum(2)}
+
+
+def _roundings(events, n, heads, kv_heads, dim, dtype, causal, v_mean=0.0, g_mean=0.0,
+               g_scale=1.0, rows=slice(None), seed=0):
+    """Root mean square error of each result over that of rounding it once."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def rand(h, mean=0.0, scale=1.0):
+        t = torch.randn(events * n, h, dim, device="cuda", generator=gen)
+        return (scale * (t + mean)).to(dtype)
+
+    q, k, v = (t.requires_grad_(True) for t in (rand(heads), rand(kv_heads),
+                                                rand(kv_heads, v_mean)))
+    g = rand(heads, g_mean, g_scale)
+    out = flash_grouped_attention_varlen(q, k, v, _offsets([n] * events), causal=causal)
+    got = dict(zip(("out", "dq", "dk", "dv"),
+                   (out.detach(),) + torch.autograd.grad(out, (q, k, v), g)))
+    by_event = lambda t: t.unflatten(0, (events, n)).transpose(1, 2)  # noqa: E731
+    want = _definition(*(by_event(t) for t in (q, k, v, g)), causal, dim**-0.5)
+    ratios = {}
+    for name, w in want.items():
+        w, x = w[:, :, rows], by_event(got[name])[:, :, rows]
+        ratios[name] = ((x.double() - w).norm() / (w.to(dtype).double() - w).norm()).item()
+    return ratios
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (FP16, 64), (BF16, 128), (BF16, 32)])
+@pytest.mark.parametrize("mean", [2.0, 8.0])
+def test_a_common_offset_of_v_leaves_the_gradients_alone(dtype, dim, causal, mean):
+    # D is that of the output whose weights sum to 1, so an offset of v cancels
+    # in dP - D. Model: 1.1 for three keys (6 and 23 with weights that do not,
+    # 4 and 15 with D from the rounded output); 1.45 for 256 (4 and 14).
+    few = _roundings(300, 3, 4, 2, dim, dtype, causal, v_mean=mean, g_mean=1.0)
+    assert few["dq"] <= 1.3 and few["dk"] <= 1.3 and few["out"] <= 1.1, few
+    more = _roundings(8, 256, 4, 2, dim, dtype, causal, v_mean=mean, g_mean=1.0)
+    assert more["dq"] <= 1.7 and more["dk"] <= 1.7 and more["out"] <= 1.1, more
+    assert few["dv"] <= 1.5 and more["dv"] <= 1.5, (few, more)
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 32), (FP16, 64), (BF16, 128)])
+def test_output_of_long_rows_with_an_offset(dtype, dim):
+    out = _roundings(1, 2500, 2, 1, dim, dtype, False, v_mean=8.0)["out"]
+    assert out <= 1.1, out
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (BF16, 128), (FP16, 32), (FP16, 64)])
+@pytest.mark.parametrize("n", [2, 3])
+def test_gradients_of_two_and_three_keys_are_rounded_about_once(dtype, dim, causal, n):
+    # Model: 1.1; 1.5 without the second part of dS; 1.9 with D from the
+    # rounded output.
+    got = _roundings(400, n, 4, 4, dim, dtype, causal, seed=n)
+    assert got["dq"] <= 1.3 and got["dk"] <= 1.3, got
