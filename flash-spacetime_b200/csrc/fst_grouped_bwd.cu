@@ -21,6 +21,16 @@
 // exponentials work at the same time on one pair of accumulators:
 //   rows:     S of the next tile | dS of this one;  dQ, next dP | next P
 //   columns:  dV, next S         | dS of this one;  dK, next dP | next P
+// fp16 ends at 6e-5 below, where dS of a long event lies (P is 1 / n, and dO is
+// small under a mean over many rows). So fp16 calls carry powers of two in P
+// and dS, folded into the exponent and the statistics at no cost a pair, and
+// taken back when the results are stored: dS of row i by the largest that
+// |dS_ij| <= 2 Dh max|dO_i| max|v_j| keeps finite in the row kernel, by one of
+// the event and key head in the column kernel, P of dV by 2^14. A short launch
+// before the two finds the maxima (16384 causal, 8 of 64: backward 1290 -> 1304
+// us). Error of dq and dk over that of one rounding, 4096 keys, Dh = 64, dO of
+// 1, 1e-2, 1e-3: 1.4, 1.4, 1.1; without 1.4, 2.8, 8.1.
+//
 // W warpgroups share a tile of 64 W rows of the other side, 64 columns each.
 // Up to Dh = 64 one group and 256 columns of tensor memory: two blocks an SM.
 // Above, dV and dK (or dQ) need twice the columns; two groups and one block,
@@ -62,6 +72,65 @@ __device__ __forceinline__ void store_rest(uint32_t dst, const float (&x)[32],
   tmem_st16(dst, w);
 }
 
+// ---- the range of fp16 ------------------------------------------------------
+
+template <typename T>
+constexpr bool scaled() {
+  return std::is_same<T, __half>::value;
+}
+constexpr int kPBits = 14;  // P <= 1 of the column kernel times 2^14
+
+// Largest |dO| and |v| of a block's 128 rows of an event and key head (all
+// query heads of the group), as fp16 bits, low and high half of the word at the
+// block's first row in ranges[kv_heads][rows].
+__global__ void __launch_bounds__(256) range_kernel(const FstGroupedBackwardArgs a, int blocks,
+                                                    uint32_t* ranges) {
+  const FstGroupedProblem& p = a.prob;
+  const int kh = blockIdx.x / blocks, group = p.heads / p.kv_heads;
+  RowTile t;
+  if (!find_tile<kBM>(p, blockIdx.x - kh * blocks, false, t) || t.i0 >= t.len) return;
+  const int vecs = p.head_dim / 8, n = min(kBM, t.len - t.i0) * vecs;
+  auto largest = [&](const FstRows& x, int h, uint32_t m) {
+    for (int e = threadIdx.x; e < n; e += 256) {
+      const uint4 w = *(const uint4*)(row_ptr<__half>(x, t, h, t.i0 + e / vecs) + e % vecs * 8);
+      m = __vmaxu2(__vmaxu2(m, __vmaxu2(w.x & 0x7fff7fff, w.y & 0x7fff7fff)),
+                   __vmaxu2(w.z & 0x7fff7fff, w.w & 0x7fff7fff));
+    }
+    return m;
+  };
+  uint32_t g = 0;
+  const uint32_t v = largest(a.v, kh, 0);
+  for (int h = kh * group; h < (kh + 1) * group; ++h) g = largest(a.dout, h, g);
+  __shared__ uint32_t warps[8];
+  const uint32_t gm = __reduce_max_sync(0xffffffffu, max(g & 0xffff, g >> 16));
+  const uint32_t vm = __reduce_max_sync(0xffffffffu, max(v & 0xffff, v >> 16));
+  if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = gm | vm << 16;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t m = 0;
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, warps[i]);
+    ranges[stat_at(p, t, p.kv_heads, kh, t.i0)] = m;
+  }
+}
+// The same of the whole event (whole warps).
+__device__ __forceinline__ uint32_t event_range(const uint32_t* ranges, const FstGroupedProblem& p,
+                                                const RowTile& t, int kh, int lane) {
+  const uint32_t* at = ranges + stat_at(p, t, p.kv_heads, kh, 0);
+  uint32_t m = 0;
+  for (int64_t i = lane * kBM; i < t.len; i += 32 * kBM) m = __vmaxu2(m, at[i]);
+  return __reduce_max_sync(0xffffffffu, m & 0xffff) |
+         __reduce_max_sync(0xffffffffu, m >> 16) << 16;
+}
+__device__ __forceinline__ float half_bits(uint32_t x) {
+  return __half2float(__ushort_as_half((unsigned short)x));
+}
+// Largest a for which 2^a 2 D g v stays below 2^15 (-26 to 62).
+__device__ __forceinline__ int power_of(int D, float g, float v) {
+  const float bound = fminf(fmaxf(2.f * D * g * v, 0x1p-47f), 0x1p40f);
+  return 15 + 126 - (__float_as_int(bound) >> 23);  // bound < 2^((bits >> 23) - 126)
+}
+__device__ __forceinline__ float exp2i(int a) { return __int_as_float((a + 127) << 23); }
+
 // ---- dq ---------------------------------------------------------------------
 
 template <int Boxes, int W, int Stages>
@@ -70,7 +139,8 @@ struct RowSmem {
   alignas(1024) char g[Boxes * kBM * 128];
   alignas(1024) char k[Stages][Boxes * W * 64 * 128];
   alignas(1024) char v[Stages][Boxes * W * 64 * 128];
-  float delta[2][kBM];  // the groups' shares of D
+  float delta[2][kBM];    // the groups' shares of D
+  uint32_t peak[2][kBM];  // and of max|dO| (fp16)
   uint64_t own_full, full[Stages], empty[Stages], s_full, s_free, dp_full, ds_ready, done;
   uint32_t tmem;
 };
@@ -78,7 +148,7 @@ struct RowSmem {
 template <typename T, int Boxes, int W, int Stages>
 __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     dq_kernel(const __grid_constant__ TileMaps maps, const FstGroupedBackwardArgs a, int blocks,
-              float* stats) {
+              float* stats, const uint32_t* ranges) {
   using Smem = RowSmem<Boxes, W, Stages>;
   extern __shared__ char raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -187,6 +257,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const bool live = i < t.len;
     const float c2 = fabsf(p.scale) * kLog2e;
     float lse2 = 0.f, delta = 0.f;
+    uint32_t range = 0, peak = 0;
+    if (scaled<T>()) range = event_range(ranges, p, t, at.kh, lane);
     if (live) {
       // Each group sums its 64 channels.
       const int d0 = w * 64, n = W == 1 ? D : min(D - d0, 64);
@@ -203,21 +275,34 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         for (int e = 0; e < 4; ++e) {
           delta = fmaf(Elem<T>::lo(xs[e]) + Elem<T>::lo(zs[e]), Elem<T>::lo(ys[e]), delta);
           delta = fmaf(Elem<T>::hi(xs[e]) + Elem<T>::hi(zs[e]), Elem<T>::hi(ys[e]), delta);
+          if (scaled<T>()) peak = __vmaxu2(peak, ys[e] & 0x7fff7fff);
         }
       }
     }
     if (W == 2) {
       sm.delta[w][row] = delta;
+      if (scaled<T>()) sm.peak[w][row] = peak;
       tc::named_sync(1, W * 128);
       delta = sm.delta[0][row] + sm.delta[1][row];
+      if (scaled<T>()) peak = __vmaxu2(sm.peak[0][row], sm.peak[1][row]);
     }
     if (live) {
       const int64_t st = stat_at(p, t, p.heads, at.h, i);
       lse2 = a.lse[st] * kLog2e;
       if (w == 0) {  // for the column kernel, in the form it adds them
-        stats[st] = -lse2;
-        stats[st + p.total_rows * p.heads] = -delta;
+        float shared = 1.f;
+        if (scaled<T>())
+          shared = exp2i(power_of(D, half_bits(range & 0xffff), half_bits(range >> 16)) - kPBits);
+        stats[st] = scaled<T>() ? kPBits - lse2 : -lse2;
+        stats[st + p.total_rows * p.heads] = -delta * shared;
       }
+    }
+    float undo = p.scale;
+    if (scaled<T>()) {
+      const int power = power_of(D, half_bits(max(peak & 0xffff, peak >> 16)),
+                                 half_bits(range >> 16));
+      lse2 -= power;
+      undo *= exp2i(-power);
     }
     const pair_t scale2 = pair(c2, c2), lse2n = pair(-lse2, -lse2), delta2n = pair(-delta, -delta);
     // One tile. `Whole`: every row of the block sees all its keys.
@@ -293,7 +378,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     // The groups share the columns of the result.
     store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr,
                  tmem + quad + 2 * kBN + w * 64, W == 1 ? D : min(D - w * 64, 64),
-                 ok ? p.scale : NAN);
+                 ok ? undo : NAN);
     tc_fence_before();
   }
   __syncthreads();
@@ -318,7 +403,7 @@ struct ColSmem {
 template <typename T, int Boxes, int W, int Stages>
 __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     dkv_kernel(const __grid_constant__ TileMaps maps, const FstGroupedBackwardArgs a, int blocks,
-               const float* stats) {
+               const float* stats, const uint32_t* ranges) {
   using Smem = ColSmem<Boxes, W, Stages>;
   extern __shared__ char raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -449,6 +534,15 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const int j = t.i0 + warp % 4 * 32 + lane;
     const float c2 = fabsf(p.scale) * kLog2e;
     const pair_t scale2 = pair(c2, c2);
+    // dS 2^power from P 2^kPBits: the factor left for dP (and, by the row
+    // kernel, for D).
+    int power = 0;
+    if (scaled<T>()) {
+      const uint32_t range = event_range(ranges, p, t, kh, lane);
+      power = power_of(D, half_bits(range & 0xffff), half_bits(range >> 16));
+    }
+    const float rest = exp2i(power - kPBits);
+    const pair_t rest2 = pair(rest, rest);
     for (int it = 0, q0 = first; it < tiles; ++it, q0 = q0 + kBN < t.len ? q0 + kBN : first) {
       const int s = it % Stages, all = min(kBN, t.len - q0);
       const int qw = q0 + w * 64, nq = t.len - qw;  // this group's columns
@@ -527,8 +621,9 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
           const ulonglong2 d4 = c ? *(const ulonglong2*)(de + c * 32 + e) : ahead[e / 4];
 #pragma unroll
           for (int f = 0; f < 4; f += 2) {
+            const pair_t p2 = pair(dp[e + f], dp[e + f + 1]), d2 = f ? d4.y : d4.x;
             const float2 y = split(mul2(pair(x[c][e + f], x[c][e + f + 1]),
-                                        add2(pair(dp[e + f], dp[e + f + 1]), f ? d4.y : d4.x)));
+                                        scaled<T>() ? fma2(p2, rest2, d2) : add2(p2, d2)));
             dp[e + f] = y.x;
             dp[e + f + 1] = y.y;
           }
@@ -557,10 +652,11 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const bool live = j < t.len;
     const uint32_t tV = tmem + quad + 2 * kBN, tK = tV + kAcc;
     if (w == 0)
-      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, tV, D, ok ? 1.f : NAN);
+      store_row<T>(live ? row_ptr<T>(a.dv, t, kh, j) : nullptr, tV, D,
+                   ok ? exp2i(scaled<T>() ? -kPBits : 0) : NAN);
     if (w == W - 1)
       store_row<T>(live ? row_ptr<T>(a.dk, t, kh, j) : nullptr, tK, D,
-                   ok ? p.scale : NAN);
+                   ok ? p.scale * exp2i(-power) : NAN);
     tc_fence_before();
   }
   __syncthreads();
@@ -599,8 +695,15 @@ int launch(const FstGroupedBackwardArgs& a, cudaStream_t st) {
   if (!rc && W == 1) rc = tc::make_rows_map(&c.v, a.v, D, rows, p.kv_heads, events, kBM);
   if (rc) return rc;
   const int blocks = (int)list_blocks(p, kBM);
-  rows_k<<<(unsigned)(blocks * p.heads), threads_of(W), row_bytes, st>>>(r, a, blocks, a.stats);
-  cols_k<<<(unsigned)(blocks * p.kv_heads), threads_of(W), col_bytes, st>>>(c, a, blocks, a.stats);
+  uint32_t* ranges = reinterpret_cast<uint32_t*>(a.stats + 2 * p.total_rows * p.heads);
+  if (scaled<T>()) {
+    range_kernel<<<(unsigned)(blocks * p.kv_heads), 256, 0, st>>>(a, blocks, ranges);
+    count_launch();
+  }
+  rows_k<<<(unsigned)(blocks * p.heads), threads_of(W), row_bytes, st>>>(r, a, blocks, a.stats,
+                                                                         ranges);
+  cols_k<<<(unsigned)(blocks * p.kv_heads), threads_of(W), col_bytes, st>>>(c, a, blocks, a.stats,
+                                                                            ranges);
   count_launch(2);
   return FST_OK;
 }

@@ -197,9 +197,10 @@ def _backward(ctx: Any, grad_out: Tensor) -> Tuple[Optional[Tensor], ...]:
     layout = ctx.layout
     dout = _in_place(grad_out)
     dq, dk, dv = (torch.empty_like(t, memory_format=_CONTIGUOUS) for t in (q, k, v))
-    stats = lse.new_empty(2 * lse.numel())
+    kv_heads, heads = _shape(k, layout, "k")[2], _shape(q, layout, "q")[2]
+    stats = lse.new_empty((2 * heads + kv_heads) * (lse.numel() // heads))
     args = _BACKWARD.pack(
-        *_problem(q, _shape(k, layout, "k")[2], layout, lens, ctx.scale, ctx.causal),
+        *_problem(q, kv_heads, layout, lens, ctx.scale, ctx.causal),
         *_rows(q, layout), *_rows(k, layout), *_rows(v, layout), *_rows(out, layout),
         *(_NO_ROWS if low is None else _rows(low, layout)), *_rows(dout, layout),
         *_rows(dq, layout), *_rows(dk, layout), *_rows(dv, layout), lse.data_ptr(), stats.data_ptr())

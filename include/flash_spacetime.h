@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define FST_ABI_VERSION 6
+#define FST_ABI_VERSION 7
 
 /* Storage dtype of q, k, v, u, wt, out, dout, dq, dk, dv. */
 enum FstDtype { FST_F32 = 0, FST_BF16 = 1, FST_F16 = 2 };
@@ -296,7 +296,8 @@ typedef struct FstGroupedBackwardArgs {
   FstRows dk;
   FstRows dv;
   const float* lse;      /* from fst_grouped_forward                         */
-  float* stats;          /* device scratch: 2 * heads * total_rows floats    */
+  float* stats;          /* device scratch: (2 * heads + kv_heads) *         */
+                         /* total_rows floats                                */
 } FstGroupedBackwardArgs;
 
 int fst_grouped_forward(const FstGroupedForwardArgs* args, void* stream);

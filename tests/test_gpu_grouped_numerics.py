@@ -154,3 +154,50 @@ def test_gradients_of_two_and_three_keys_are_rounded_about_once(dtype, dim, caus
     # rounded output.
     got = _roundings(400, n, 4, 4, dim, dtype, causal, seed=n)
     assert got["dq"] <= 1.3 and got["dk"] <= 1.3, got
+
+
+@pytest.mark.parametrize("g_scale", [1.0, 1e-2, 1e-3])
+@pytest.mark.parametrize("dim, causal", [(64, False), (64, True), (32, False), (128, True),
+                                         (100, False)])
+def test_fp16_gradients_of_long_events_keep_their_small_values(dim, causal, g_scale):
+    # dS is about 1 / n of its row's gradient and falls below the normal range
+    # of fp16 long before dq does. Model: 1.4; 2.8 (1e-2) and 8 (1e-3) with dS
+    # in fp16 as it is.
+    got = _roundings(1, 4096, 2, 1, dim, FP16, causal, g_scale=g_scale)
+    assert got["dq"] <= 1.6 and got["dk"] <= 1.6 and got["dv"] <= 1.6, got
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_fp16_gradients_do_not_depend_on_other_events(dim):
+    # Two events whose gradients are 2^12 apart, and an infinity in a third: each
+    # has the bits that it has alone.
+    lens, heads = [700, 1500, 40], 4
+    leaves, g = _packed(lens, heads, 2, dim, FP16)
+    g[700:2200] *= 2.0**-12
+    g[2210] = float("inf")
+    cu = _offsets(lens)
+    out = flash_grouped_attention_varlen(*leaves, cu)
+    all_events = torch.autograd.grad(out, leaves, g)
+    for a, b in ((0, 700), (700, 2200)):
+        own = [t.detach()[a:b].clone().requires_grad_(True) for t in leaves]
+        out = flash_grouped_attention_varlen(*own, _offsets([b - a]))
+        for x, y in zip(torch.autograd.grad(out, own, g[a:b]), all_events):
+            assert torch.equal(x, y[a:b])
+            assert x.isfinite().all() and x.count_nonzero() > 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_fp16_gradients_of_large_values_are_finite(dim):
+    # |dS| reaches 1e6, far past fp16; dq and dk, with a small scale, do not.
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v, g = (s * torch.randn(2, 2, 300, dim, device="cuda", generator=gen)
+                  for s in (1, 1, 64, 512))
+    leaves = [t.half().requires_grad_(True) for t in (q, k, v)]
+    g = g.half()
+    out = flash_grouped_attention(*leaves, scale=2.0**-9)
+    got = torch.autograd.grad(out, leaves, g)
+    want = _definition(*leaves, g, True, 2.0**-9)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        w = want[name]
+        assert x.isfinite().all() and w.abs().max() < 65504
+        assert (x.double() - w).norm() <= 1.6 * (w.half().double() - w).norm()
