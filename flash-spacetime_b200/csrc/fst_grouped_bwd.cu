@@ -57,11 +57,18 @@ constexpr int kBM = 128;  // rows a block owns
 constexpr int threads_of(int W) { return W * 128 + 64; }
 constexpr int resident_of(int W) { return W == 1 ? 2 : 1; }
 
-// Events of so few rows take dS in two 16-bit parts, and one more product. With
-// two keys dS_1 = -dS_2, and its rounding goes into dq whole (1.6 times the
-// error of rounding dq itself); over more keys the roundings average out (1.4
-// times from 4 keys on, however many).
-constexpr int kFew = 32;
+// Rows that see at most kFew keys take dS in two 16-bit parts, and one more
+// product: all rows of an event of so few, the first ones of a causal event.
+// With two keys dS_1 = -dS_2, and its rounding goes into dq whole; over more keys
+// the roundings average out (error of dq over that of rounding dq itself: rows 1
+// to 3 of a causal event 1.5, with the second part 1.1; from some 30 keys on 1.4
+// whatever their number). Only the first tile of a block holds such rows, and only
+// its first 32 keys (columns: query rows) need the second part: it lies between
+// the first parts of those and of the next 32, which move up by kFewGap columns.
+constexpr int kFew = 32, kFewGap = 16;
+__device__ __forceinline__ bool few_keys(const FstGroupedProblem& p, const RowTile& t) {
+  return t.len <= kFew || (p.causal && t.i0 == 0);
+}
 template <typename T>
 __device__ __forceinline__ void store_rest(uint32_t dst, const float (&x)[32],
                                            const uint32_t (&rounded)[16]) {
@@ -216,7 +223,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const int n = uniform(tiles), last = uniform(end), dim = uniform(D);
     const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, q_mem = p_mem + kBN;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
-    const bool few = uniform(t.len) <= kFew;  // one tile then
+    const bool few = uniform(few_keys(p, t));
     auto keys = [&](int it) { return min(kBN, last - it * kBN); };
     auto logits = [&](int it) {
       if (!mbar_wait(smem_addr(&sm.full[it % Stages]), (it / Stages) & 1)) return false;
@@ -242,9 +249,12 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       ok = ok && mbar_wait(smem_addr(&sm.ds_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
+      const bool second = few && it == 0;
       accumulate<kBN>(q_mem, p_mem, smem_addr(sm.k[it % Stages]), keys(it), acc_instr, it > 0,
-                      leader);
-      if (few) accumulate<kBN>(q_mem, p_mem + 32, smem_addr(sm.k[0]), last, acc_instr, true, leader);
+                      leader, second ? kFewGap : 0);
+      if (second)
+        accumulate<kBN>(q_mem, p_mem + kFewGap, smem_addr(sm.k[0]), min(last, kFew), acc_instr,
+                        true, leader);
       tc_commit(smem_addr(&sm.empty[it % Stages]), leader);
       if (it + 1 < n) weights(it + 1);
     }
@@ -335,6 +345,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       const int keys = p.causal ? min(i + 1, t.len) : t.len;
       const int lim = (keys > 1 ? keys : 0) - j0;
       const int fewest = Whole ? 64 : uniform(lim);
+      const bool second = Few && w == 0;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (!Whole && c * 32 >= nk) continue;
@@ -356,8 +367,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         uint32_t x[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = Elem<T>::pack(dp[2 * e], dp[2 * e + 1]);
-        tmem_st16(tP + c * 16, x);
-        if (Few && c == 0) store_rest<T>(tP + 32, dp, x);
+        tmem_st16(tP + c * (second ? 16 + kFewGap : 16), x);
+        if (second && c == 0) store_rest<T>(tP + kFewGap, dp, x);
       }
       const int all = min(kBN, end - it * kBN);
       if (!Whole && (all & 15))  // dS is 0 there, and must not meet another event's NaN
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const int whole = min(tiles, (p.causal ? min(t.len, t.i0 + 1) : t.len) / kBN);
     int it = 0;
     for (; it < whole && ok; ++it) ok = tile(std::true_type(), std::false_type(), it);
-    if (t.len <= kFew) ok = tile(std::false_type(), std::true_type(), it++);
+    if (few_keys(p, t)) ok = tile(std::false_type(), std::true_type(), it++);
     for (; it < tiles && ok; ++it) ok = tile(std::false_type(), std::false_type(), it);
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
@@ -489,7 +500,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, v_mem = p_mem + kBN,
                    k_mem = v_mem + kAcc;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
-    const bool few = uniform(t.len) <= kFew;  // one tile a head then
+    const bool few = uniform(few_keys(p, t));
     // S^T over P^T and dP^T over dS^T: MMAs complete in order, so the products
     // that read those are done.
     auto logits = [&](int it, int q_rows) {
@@ -509,6 +520,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     if (ok) weights(0, q_rows);
     for (int it = 0; it < n && ok; ++it) {
       const int s = it % Stages;
+      const bool second = few && done == 0;  // a head's first tile
       done = done + kBN < rows ? done + kBN : 0;
       const int next_rows = min(kBN, rows - done);
       ok = mbar_wait(smem_addr(&sm.p_ready), it & 1);
@@ -519,9 +531,11 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       ok = ok && mbar_wait(smem_addr(&sm.ds_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
-      accumulate<kBN>(k_mem, p_mem, smem_addr(sm.q[s]), q_rows, acc_instr, it > 0, leader);
-      if (few)
-        accumulate<kBN>(k_mem, p_mem + 32, smem_addr(sm.q[s]), q_rows, acc_instr, true, leader);
+      accumulate<kBN>(k_mem, p_mem, smem_addr(sm.q[s]), q_rows, acc_instr, it > 0, leader,
+                      second ? kFewGap : 0);
+      if (second)
+        accumulate<kBN>(k_mem, p_mem + kFewGap, smem_addr(sm.q[s]), min(q_rows, kFew), acc_instr,
+                        true, leader);
       tc_commit(smem_addr(&sm.empty[s]), leader);
       if (it + 1 < n) weights(it + 1, next_rows);
       q_rows = next_rows;
@@ -609,6 +623,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       ok = mbar_wait(smem_addr(&sm.dp_full), it & 1);
       if (!ok) break;
       tc_fence_after();
+      const bool second = w == 0 && q0 == first && few_keys(p, t);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (c * 32 >= nq) continue;
@@ -638,8 +653,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         uint32_t y[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = Elem<T>::pack(dp[2 * e], dp[2 * e + 1]);
-        tmem_st16(tP + c * 16, y);
-        if (c == 0 && t.len <= kFew) store_rest<T>(tP + 32, dp, y);
+        tmem_st16(tP + c * (second ? 16 + kFewGap : 16), y);
+        if (second && c == 0) store_rest<T>(tP + kFewGap, dp, y);
       }
       tmem_wait_st();
       tc_fence_before();

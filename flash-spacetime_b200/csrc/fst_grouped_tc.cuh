@@ -281,16 +281,17 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t A, uint32_t B, int 
 }
 // d[128][n] (+)= P X over `rows` rows (rounded up to 16) of X, a tile of BRows
 // rows; P 16-bit values in tensor memory, 64 rows of X in 32 columns, the
-// next 64 from 64 columns on. XStep: bytes of 16 rows of X (0: the same rows
-// every time).
+// next 64 from 64 columns on; `gap` columns between the first 32 rows' and the
+// next 32's. XStep: bytes of 16 rows of X (0: the same rows every time).
 template <int BRows, int XStep = 2048>
 __device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, int rows,
-                                           uint32_t instr, bool add, uint32_t leader) {
+                                           uint32_t instr, bool add, uint32_t leader,
+                                           uint32_t gap = 0) {
   const uint64_t x = operand(X, BRows * 128);
 #pragma unroll
   for (int c = 0; c < BRows / 16; ++c)
     if (c * 16 < rows)
-      mma_ts(d, P + c / 4 * 64 + c % 4 * 8, x + c * XStep / 16, instr, add || c > 0, leader);
+      mma_ts(d, P + c / 4 * 64 + c % 4 * 8 + (c == 2 || c == 3 ? gap : 0), x + c * XStep / 16, instr, add || c > 0, leader);
 }
 
 // The block's rows of no event: zeros, in 16-byte vectors, by n threads.

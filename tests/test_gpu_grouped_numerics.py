@@ -201,3 +201,15 @@ def test_fp16_gradients_of_large_values_are_finite(dim):
         w = want[name]
         assert x.isfinite().all() and w.abs().max() < 65504
         assert (x.double() - w).norm() <= 1.6 * (w.half().double() - w).norm()
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (BF16, 128), (FP16, 32), (FP16, 128)])
+@pytest.mark.parametrize("n", [32, 33, 64, 65, 200, 300])
+def test_first_rows_of_causal_events_are_rounded_about_once(dtype, dim, n):
+    # Rows that see few keys, whatever the event's length. Model: 1.1; 1.5
+    # without the second part of dS.
+    got = _roundings(100, n, 4, 2, dim, dtype, True, rows=slice(1, 4), seed=n)
+    assert got["dq"] <= 1.3, got
+    if n <= 33:
+        got = _roundings(100, n, 4, 2, dim, dtype, True, seed=n)
+        assert got["dq"] <= 1.3 and got["dk"] <= 1.3, got
