@@ -150,7 +150,10 @@ struct Shape {
   int rows, groups, heads, slots;
 };
 
-template <typename T, int V, bool Interleaved>
+// Events: positions come from cu_seqlens, so rows may belong to no event. Those
+// keep their bits: an infinity or NaN would not survive x * 1 - y * 0. (A variant
+// of its own: asked of padded fp32 rows, the question costs 4 %, in spills.)
+template <typename T, int V, bool Interleaved, bool Events>
 __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(FstRotaryArgs p, Shape sh) {
   __shared__ float2 table[kMaxTable];
   __shared__ double pos[kMaxRows];
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(FstRotaryArgs p, Sh
     const int u = u0 + threadIdx.x, gr = u / sh.slots, r = gr / sh.groups;
     const int g = gr - r * sh.groups;
     const bool mine = u < units;
-    const Slot t = slot_at<V, Interleaved>(p, u - gr * sh.slots);
+    Slot t = slot_at<V, Interleaved>(p, u - gr * sh.slots);
     int64_t ev = ev0, i = i0 + r;
     while (mine && !p.packed && i >= p.max_len) {
       i -= p.max_len;
@@ -214,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(FstRotaryArgs p, Sh
         __syncthreads();
       }
       if (!mine) continue;
+      if (Events && h0 == g && !live[r]) t.pair = -1;
       if (h0 == g && t.pair >= 0) {
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -264,8 +268,12 @@ int launch(const FstRotaryArgs& p, cudaStream_t st) {
     return api_fail(FST_ERR_UNSUPPORTED, "rotary: %lld rows are too many",
                     (long long)p.total_rows);
   const Shape sh{rows, groups, heads, slots};
-  const auto kernel = vec ? (p.interleaved ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>)
-                          : (p.interleaved ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
+  const bool events = p.packed && !p.positions;
+  const auto kernel =
+      vec ? (p.interleaved ? (events ? rotary_kernel<T, V, true, true> : rotary_kernel<T, V, true, false>)
+                           : (events ? rotary_kernel<T, V, false, true> : rotary_kernel<T, V, false, false>))
+          : (p.interleaved ? (events ? rotary_kernel<T, 1, true, true> : rotary_kernel<T, 1, true, false>)
+                           : (events ? rotary_kernel<T, 1, false, true> : rotary_kernel<T, 1, false, false>));
   kernel<<<(unsigned)blocks, kThreads, 0, st>>>(p, sh);
   count_launch();
   return FST_OK;

@@ -221,3 +221,27 @@ def test_gradient_against_differences():
                - flash_rotary_varlen(q, None, freqs, cu)[0].double())
     want = (far * w.double()).sum()
     assert abs((dq.double() * d.double()).sum() - want) <= 2.0**-20 * 240 * 16
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype, dim, rot", [(BF16, 32, 32), (FP32, 64, 32), (FP16, 10, 6),
+                                             (FP32, 7, 6), (BF16, 24, 16)])
+def test_rows_of_no_event_keep_their_bits(dtype, dim, rot, interleaved):
+    # Whatever such rows hold: infinities, NaN and zeros of either sign, whose
+    # partner a rotation by 0 would change (x * 1 - y * 0).
+    x = torch.randn(40, 3, dim, device="cuda").to(dtype)
+    odd = torch.tensor([float("inf"), float("-inf"), float("nan"), -0.0, 0.0, 1.0], device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    dead = torch.tensor([0, 1, 2, 30, 31, 39], device="cuda")
+    pick = torch.randint(6, (6, 3, dim), device="cuda", generator=gen)
+    x[dead] = odd[pick].to(dtype)
+    cu = torch.tensor([3, 9, 30], dtype=torch.int32, device="cuda")
+    bits = {2: torch.int16, 4: torch.int32}[x.element_size()]
+    freqs = rotary_frequencies(rot)
+    got, _ = flash_rotary_varlen(x, None, freqs, cu, interleaved=interleaved, magnitude=2.0)
+    assert torch.equal(got[dead].view(bits), x[dead].view(bits))
+    _check(got[3:30], x[3:30], freqs, _event_positions([6, 21])[:, None], interleaved, 2.0)
+    leaf = torch.zeros_like(x).requires_grad_(True)
+    out, _ = flash_rotary_varlen(leaf, None, freqs, cu, interleaved=interleaved)
+    (grad,) = torch.autograd.grad(out, leaf, x)
+    assert torch.equal(grad[dead].view(bits), x[dead].view(bits))
