@@ -232,7 +232,8 @@ def rotary_frequencies(
     * ``"parts"``: pairs that turn ``fast_turns`` times or more over
       ``trained_len`` keep their frequency, those that turn ``slow_turns``
       times or less are divided by the factor, a ramp linear in the turns
-      between (used with ``rotary_magnitude(factor)``).
+      between (used with ``rotary_magnitude(factor)``). A model trained with a
+      ramp linear in the channel index needs that model's own frequencies.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim (={rotary_dim}) must be even and at least 2")

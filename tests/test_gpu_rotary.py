@@ -6,6 +6,9 @@ sincospi, times the magnitude m), rounded once: the bound is
 u |ref| + 2^-21 m (|x| + |y|), u half a step of the type.
 """
 
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -245,3 +248,41 @@ def test_rows_of_no_event_keep_their_bits(dtype, dim, rot, interleaved):
     out, _ = flash_rotary_varlen(leaf, None, freqs, cu, interleaved=interleaved)
     (grad,) = torch.autograd.grad(out, leaf, x)
     assert torch.equal(grad[dead].view(bits), x[dead].view(bits))
+
+
+def _pi():
+    """pi as a fraction, to 100 decimals: 16 atan(1/5) - 4 atan(1/239)."""
+    unit = 10**110
+
+    def atan(x):
+        total, term, n = 0, unit // x, 1
+        while term:
+            total += term // n if n % 4 == 1 else -(term // n)
+            term, n = term // (x * x), n + 2
+        return total
+
+    return Fraction(16 * atan(5) - 4 * atan(239), unit)
+
+
+@pytest.mark.parametrize("start", [0, 10**6, 2**28, 2**31 - 20, 2**32, 2**40 + 3, 2**47 + 1])
+def test_angles_against_exact_arithmetic(start):
+    # Rows (1, 0) come back as (cos, sin) of position * freq, here in exact
+    # rational arithmetic: within the 2^-22 of this file's header and the stated
+    # 3 * 2^-53 of the angle.
+    gen = torch.Generator().manual_seed(7)
+    freqs = torch.cat((0.5 + torch.rand(24, generator=gen, dtype=torch.float64),
+                       rotary_frequencies(16)))
+    half = freqs.numel()
+    pos = start + torch.arange(40)
+    x = torch.zeros(40, 1, 2 * half, device="cuda")
+    x[..., :half] = 1
+    got, _ = flash_rotary_varlen(x, None, freqs, positions=pos.cuda())
+    got = got[:, 0].double().cpu()
+    two_pi = 2 * _pi()
+    for i in range(40):
+        for j in range(half):
+            turns = int(pos[i]) * Fraction(freqs[j].item()) / two_pi
+            angle = 2 * math.pi * float(turns - round(turns))
+            bound = 2.0**-22 + 3 * 2.0**-53 * 2 * math.pi * float(turns)
+            assert abs(got[i, j] - math.cos(angle)) <= bound
+            assert abs(got[i, half + j] - math.sin(angle)) <= bound
