@@ -86,6 +86,25 @@ def _integers(t: Tensor, what: str) -> Tensor:
     return t
 
 
+def _bool_mask(mask: Any, shape: Tuple[int, int], validate: bool) -> Any:
+    """A 2-D padding mask as bool (True: padding); anything else as it is. A float
+    mask marks padding with -inf or its type's lowest value, valid rows with 0."""
+    if not isinstance(mask, Tensor) or mask.dim() != 2:
+        return mask
+    if mask.shape != shape:
+        raise ValueError(f"a padding mask must be [B, L] = [{shape[0]}, {shape[1]}], got "
+                         f"{tuple(mask.shape)}")
+    if mask.dtype == torch.bool:
+        return mask
+    if not mask.dtype.is_floating_point:
+        raise ValueError(f"a padding mask must be bool or float, got {mask.dtype}")
+    padding = mask <= torch.finfo(mask.dtype).min
+    if validate and bool((~padding & (mask != 0)).any()):
+        raise ValueError("a float padding mask must be 0 (valid) or -inf or its type's lowest "
+                         "value (padding) everywhere")
+    return padding
+
+
 def _shape(t: Tensor, layout: str, what: str) -> Sizes:
     """(events, rows per event or in all, heads, Dh) of a tensor."""
     shape = t.shape
@@ -255,7 +274,9 @@ def flash_grouped_attention(
     Dh at most 128 (fp32, bf16 or fp16); with ``layout='blhd'`` all are
     ``[B, L, heads, Dh]``. ``seqlens`` is the ``[B]`` valid prefix lengths
     (on any device, or a list; clamped to ``[0, L]``) or a ``[B, L]`` padding mask, as for
-    :func:`flash_spacetime_attention`; None means that every row is valid.
+    :func:`flash_spacetime_attention`, whose float form may also mark padding
+    with its type's lowest value; None means that every row is valid. Integer
+    masks are refused, and with ``validate_mask`` other float values.
     ``scale`` multiplies the logits (default ``Dh**-0.5``). With ``causal``
     row i sees the rows j <= i of its event, else all of them.
 
@@ -267,10 +288,8 @@ def flash_grouped_attention(
     events, rows, _, _ = _check_heads(q, k, v, layout)
     if isinstance(seqlens, Tensor) and seqlens.dim() == 1:
         _integers(seqlens, "seqlens")
-    for mask in (seqlens, key_padding_mask):
-        if isinstance(mask, Tensor) and mask.dim() == 2 and mask.shape != (events, rows):
-            raise ValueError(f"a padding mask must be [B, L] = [{events}, {rows}], got "
-                             f"{tuple(mask.shape)}")
+    seqlens, key_padding_mask = (_bool_mask(m, (events, rows), validate_mask)
+                                 for m in (seqlens, key_padding_mask))
     lens, _ = _padded_lengths(seqlens, key_padding_mask, events, rows, q.device, validate_mask,
                               None)
     lens = _integers(torch.as_tensor(lens), "seqlens")
