@@ -86,6 +86,17 @@ def _integers(t: Tensor, what: str) -> Tensor:
     return t
 
 
+def _int32(t: Tensor, most: int, device: torch.device) -> Tensor:
+    """``t`` as int32 on ``device``; wider types are clamped to [0, most], so
+    that nothing wraps (the kernels clamp int32 themselves)."""
+    if t.dtype == torch.uint64:  # above 2^63 - 1 as an int64: negative
+        t = t.to(torch.int64)
+        t = torch.where(t < 0, torch.full_like(t, most), t)
+    if t.dtype in (torch.int64, torch.uint32):
+        t = t.to(torch.int64).clamp(0, most)
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 def _bool_mask(mask: Any, shape: Tuple[int, int], validate: bool) -> Any:
     """A 2-D padding mask as bool (True: padding); anything else as it is. A float
     mask marks padding with -inf or its type's lowest value, valid rows with 0."""
@@ -292,10 +303,10 @@ def flash_grouped_attention(
                                  for m in (seqlens, key_padding_mask))
     lens, _ = _padded_lengths(seqlens, key_padding_mask, events, rows, q.device, validate_mask,
                               None)
-    lens = _integers(torch.as_tensor(lens), "seqlens")
-    if lens.dtype == torch.int64:  # must not wrap into 32 bits; the kernels clamp the rest
-        lens = lens.clamp(0, rows)
-    lens = lens.to(device=q.device, dtype=torch.int32).contiguous()
+    if not isinstance(lens, Tensor):
+        lens = torch.as_tensor(lens)
+        lens = lens if lens.numel() else lens.to(torch.int64)  # an empty list has no type
+    lens = _int32(_integers(lens, "seqlens"), rows, q.device)
     if lens.shape != (events,):
         raise ValueError(f"seqlens must be [B] = [{events}], got {tuple(lens.shape)}")
     return _apply(q, k, v, lens, layout, scale, causal)
@@ -321,8 +332,5 @@ def flash_grouped_attention_varlen(
     _check_heads(q, k, v, "packed")
     if not isinstance(cu_seqlens, Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens must be a [B+1] tensor")
-    cu = _integers(cu_seqlens, "cu_seqlens")
-    if cu.dtype == torch.int64:
-        cu = cu.clamp(0, q.shape[0])
-    cu = cu.to(device=q.device, dtype=torch.int32).contiguous()
+    cu = _int32(_integers(cu_seqlens, "cu_seqlens"), q.shape[0], q.device)
     return _apply(q, k, v, cu, "packed", scale, causal)

@@ -13,8 +13,8 @@ from typing import Any, Optional, Tuple
 import torch
 from torch import Tensor
 
-from .grouped import (_CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _integers, _rows, _shape,
-                      once, seen_by_autograd)
+from .grouped import (_CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _int32, _integers,
+                      _rows, _shape, once, seen_by_autograd)
 from .ops import _DTYPES
 
 _ROTARY = struct.Struct("@11ifq3Q" + 4 * _ROWS)
@@ -107,8 +107,8 @@ def _apply(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
             positions = positions.expand(want)
         if tuple(positions.shape) != want:
             raise ValueError(f"positions must be {list(want)}, got {list(positions.shape)}")
-        if positions.dtype not in (torch.int32, torch.int64):
-            positions = positions.to(torch.int32)
+        if positions.dtype != torch.int32:
+            positions = positions.to(torch.int64)
         positions = positions.to(q.device).contiguous()
     args = (q, k, freqs, cu, positions, layout, bool(interleaved), float(magnitude))
     if seen_by_autograd(q, k):
@@ -167,7 +167,5 @@ def flash_rotary_varlen(
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
             raise ValueError("cu_seqlens must be a [B+1] tensor")
         cu = _integers(cu_seqlens, "cu_seqlens")
-        if cu.dtype == torch.int64:
-            cu = cu.clamp(0, 2**31 - 1)
-        cu = cu.to(device=q.device, dtype=torch.int32).contiguous()
+        cu = _int32(cu, 2**31 - 1, q.device)
     return _apply(q, k, freqs, cu, positions, "packed", interleaved, magnitude)
