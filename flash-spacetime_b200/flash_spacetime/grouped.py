@@ -81,6 +81,8 @@ def _rows(t: Tensor, layout: str) -> Tuple[int, int, int, int]:
 
 
 def _integers(t: Tensor, what: str) -> Tensor:
+    if not isinstance(t, Tensor):
+        raise ValueError(f"{what} must be a tensor of integers, got {type(t).__name__}")
     if t.dtype == torch.bool or t.dtype.is_floating_point or t.dtype.is_complex:
         raise ValueError(f"{what} must be integers, got {t.dtype}")
     return t
@@ -95,6 +97,13 @@ def _int32(t: Tensor, most: int, device: torch.device) -> Tensor:
     if t.dtype in (torch.int64, torch.uint32):
         t = t.to(torch.int64).clamp(0, most)
     return t.to(device=device, dtype=torch.int32).contiguous()
+
+
+def _finite_fp32(x: float, what: str) -> float:
+    x = float(x)
+    if not abs(x) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"{what} must be finite in fp32, got {x}")
+    return x
 
 
 def _bool_mask(mask: Any, shape: Tuple[int, int], validate: bool) -> Any:
@@ -255,13 +264,15 @@ def _check_heads(q: Tensor, k: Tensor, v: Tensor, layout: str) -> Sizes:
         raise ValueError(f"the heads of q ({heads}) must be a multiple of those of k ({kv_heads})")
     if not 1 <= dim <= 128:
         raise ValueError(f"Dh (={dim}) must be 1 to 128")
+    if max(1, events) * rows >= 2**31 - 255:
+        raise ValueError(f"q has {max(1, events) * rows} rows, at most {2**31 - 256} are supported")
     return sizes
 
 
 def _apply(q: Tensor, k: Tensor, v: Tensor, lens: Tensor, layout: str, scale: Optional[float],
            causal: bool) -> Tensor:
-    args = (q, k, v, lens, layout, float(q.shape[-1]**-0.5 if scale is None else scale),
-            bool(causal))
+    args = (q, k, v, lens, layout,
+            _finite_fp32(q.shape[-1]**-0.5 if scale is None else scale, "scale"), bool(causal))
     if seen_by_autograd(q, k, v):
         return _FlashGroupedAttention.apply(*args)
     return _forward(*args)[0]

@@ -13,8 +13,8 @@ from typing import Any, Optional, Tuple
 import torch
 from torch import Tensor
 
-from .grouped import (_CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _int32, _integers,
-                      _rows, _shape, once, seen_by_autograd)
+from .grouped import (_CONTIGUOUS, _NO_ROWS, _ROWS, _call, _check_tensor, _finite_fp32, _int32,
+                      _integers, _rows, _shape, once, seen_by_autograd)
 from .ops import _DTYPES
 
 _ROTARY = struct.Struct("@11ifq3Q" + 4 * _ROWS)
@@ -94,6 +94,10 @@ def _apply(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
             raise ValueError("k has no heads (pass k=None)")
     if heads < 1 or not 1 <= dim <= 1024:
         raise ValueError(f"q must have heads of 1 to 1024 channels, got {tuple(q.shape)}")
+    if not isinstance(freqs, Tensor):
+        raise ValueError(f"freqs must be a tensor, got {type(freqs).__name__}")
+    if layout != "packed" and rows >= 2**31:
+        raise ValueError(f"{rows} rows an event: at most {2**31 - 1}")
     if freqs.dim() != 1 or not freqs.dtype.is_floating_point or 2 * freqs.numel() > dim:
         raise ValueError(f"freqs must be [R/2] floats with R <= Dh (={dim}), got "
                          f"{tuple(freqs.shape)} {freqs.dtype}")
@@ -110,7 +114,8 @@ def _apply(q: Tensor, k: Optional[Tensor], freqs: Tensor, cu: Optional[Tensor],
         if positions.dtype != torch.int32:
             positions = positions.to(torch.int64)
         positions = positions.to(q.device).contiguous()
-    args = (q, k, freqs, cu, positions, layout, bool(interleaved), float(magnitude))
+    args = (q, k, freqs, cu, positions, layout, bool(interleaved),
+            _finite_fp32(magnitude, "magnitude"))
     if seen_by_autograd(q, k):
         return _FlashRotary.apply(*args)
     return _rotate(*args, False)
@@ -164,8 +169,8 @@ def flash_rotary_varlen(
     if positions is None:
         if cu_seqlens is None:
             raise ValueError("pass cu_seqlens or positions")
-        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
-            raise ValueError("cu_seqlens must be a [B+1] tensor")
         cu = _integers(cu_seqlens, "cu_seqlens")
+        if cu.dim() != 1 or cu.numel() < 1:
+            raise ValueError("cu_seqlens must be a [B+1] tensor")
         cu = _int32(cu, 2**31 - 1, q.device)
     return _apply(q, k, freqs, cu, positions, "packed", interleaved, magnitude)

@@ -96,6 +96,11 @@ def test_offsets(seen):
         flash_grouped_attention_varlen(q, k, k, cu)
         flash_rotary_varlen(q, k, FREQS, cu)
     assert all(x[:2] == [0, 4] and x[2] >= 6 for x in seen) and len(seen) == 8
+    for bad in ([0, 6], None, torch.tensor(6), torch.tensor([0.0, 6.0]), torch.zeros(0).long()):
+        with pytest.raises(ValueError):
+            flash_grouped_attention_varlen(q, k, k, bad)
+        with pytest.raises(ValueError):
+            flash_rotary_varlen(q, k, FREQS, bad)
 
 
 def test_positions_of_unsigned_types(seen):
@@ -104,3 +109,28 @@ def test_positions_of_unsigned_types(seen):
                        (torch.int64, 2**40), (torch.int32, -1)):
         flash_rotary_varlen(q, k, FREQS, positions=torch.tensor([3, far], dtype=dtype))
         assert seen[-1] == [3, far]
+    for bad in ([3, 4], torch.tensor([3.0, 4.0])):
+        with pytest.raises(ValueError):
+            flash_rotary_varlen(q, k, FREQS, positions=bad)
+
+
+@pytest.mark.parametrize("value", [1e39, -1e39, float("inf"), float("nan")])
+def test_scalars_past_fp32_are_refused(seen, value):
+    q, k = _padded(1)
+    with pytest.raises(ValueError, match="finite"):
+        flash_grouped_attention(q, k, k, scale=value)
+    with pytest.raises(ValueError, match="finite"):
+        flash_rotary(q, k, FREQS, magnitude=value)
+    with pytest.raises(ValueError, match="freqs"):
+        flash_rotary(q, k, [1.0, 0.1])
+    assert not seen
+
+
+def test_row_counts_past_32_bits_are_refused(seen):
+    q = torch.zeros(1).expand(2, 1, 2**30, 8)
+    with pytest.raises(ValueError, match="rows"):
+        flash_grouped_attention(q, q, q)
+    q = torch.zeros(1).expand(1, 1, 2**31, 8)
+    with pytest.raises(ValueError, match="rows"):
+        flash_rotary(q, q, FREQS)
+    assert not seen
