@@ -167,7 +167,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
       // Asked for only now, with the item's last loads under way, so that no
-      // block holds work that another has time for.
+      // block holds work that another has time for. After a wait that ran out,
+      // not at all: what is asked for would be lost, its rows left as they were.
+      if (!ok) break;
       if (lane == 0) feed_ask(sm.feed);
       __syncwarp();
       index = feed_answer(sm.feed, round);
