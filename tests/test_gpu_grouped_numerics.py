@@ -7,7 +7,9 @@ import torch
 pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
-    from flash_spacetime import flash_grouped_attention, flash_grouped_attention_varlen
+    from flash_spacetime import (flash_grouped_attention, flash_grouped_attention_varlen,
+                                 flash_rotary_varlen, grouped_attention_reference,
+                                 rotary_frequencies, rotary_reference)
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 # Tensor cores (one and two boxes of channels, a head that ends inside one), CUDA cores.
@@ -213,3 +215,70 @@ def test_first_rows_of_causal_events_are_rounded_about_once(dtype, dim, n):
     if n <= 33:
         got = _roundings(100, n, 4, 2, dim, dtype, True, seed=n)
         assert got["dq"] <= 1.3 and got["dk"] <= 1.3, got
+
+
+# Sizes past those of the elementwise tests: long events, and enough of them
+# that each block of the forward works through many.
+
+
+@pytest.mark.parametrize("n, causal", [(5000, False), (9001, True)])
+@pytest.mark.parametrize("dtype, dim, heads, kv_heads", [(BF16, 32, 2, 2), (FP16, 64, 2, 1),
+                                                         (BF16, 128, 2, 1)])
+def test_long_events(dtype, dim, heads, kv_heads, n, causal):
+    # Model: out 1.4, dq and dk 1.45, dv 1.45 (over many keys P and dS are
+    # rounded as often as the results).
+    got = _roundings(1, n, heads, kv_heads, dim, dtype, causal)
+    assert max(got.values()) <= 1.6, got
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 32), (FP16, 64), (BF16, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_events(dtype, dim, causal):
+    # 7200 items of the forward, some 25 to a block.
+    got = _roundings(300, 130, 12, 4, dim, dtype, causal)
+    assert max(got.values()) <= 1.6, got
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 32), (FP16, 64), (BF16, 128), (FP32, 32)])
+def test_an_event_has_the_same_bits_wherever_it_lies(dtype, dim):
+    gen = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 400, (500,), generator=gen).tolist()
+    leaves, g = _packed(lens, 6, 2, dim, dtype)
+    starts = _offsets(lens)[:-1].tolist()
+    order = torch.randperm(500, generator=gen).tolist()
+    rows = torch.cat([torch.arange(starts[e], starts[e] + lens[e]) for e in order]).cuda()
+
+    def run(leaves, g, lens):
+        out = flash_grouped_attention_varlen(*leaves, _offsets(lens))
+        return (out.detach(),) + torch.autograd.grad(out, leaves, g)
+
+    moved = [t.detach()[rows].requires_grad_(True) for t in leaves]
+    for a, b in zip(run(leaves, g, lens), run(moved, g[rows], [lens[e] for e in order])):
+        assert torch.equal(a[rows], b)
+
+
+@pytest.mark.parametrize("dtype, tol", [(BF16, 2e-2), (FP32, 1e-5)])
+def test_rotary_then_attention_event_by_event(dtype, tol):
+    # The two ops as they are used, each result of each event within the package's
+    # parity tolerance of its own size; one row has no gradient of q and k.
+    lens, heads, kv_heads, dim = [140, 1, 2, 263], 6, 2, 64
+    (q, k, v), g = _packed(lens, heads, kv_heads, dim, dtype, seed=5)
+    freqs, cu = rotary_frequencies(32), _offsets(lens)
+    qr, kr = flash_rotary_varlen(q, k, freqs, cu)
+    out = flash_grouped_attention_varlen(qr, kr, v, cu)
+    got = (out.detach(),) + torch.autograd.grad(out, (q, k, v), g)
+    at = 0
+    for n in lens:
+        ref = [t.detach()[at:at + n].double().transpose(0, 1)[None].cpu().requires_grad_(True)
+               for t in (q, k, v)]
+        pos = torch.arange(n)[None, None]
+        o = grouped_attention_reference(rotary_reference(ref[0], freqs, pos),
+                                        rotary_reference(ref[1], freqs, pos), ref[2])
+        grads = torch.autograd.grad(o, ref, g[at:at + n].double().transpose(0, 1)[None].cpu())
+        for i, (a, b) in enumerate(zip(got, (o.detach(),) + grads)):
+            a = a[at:at + n].transpose(0, 1).double().cpu()
+            if n == 1 and i in (1, 2):
+                assert a.count_nonzero() == 0
+            else:
+                assert (a - b[0]).norm() <= tol * b.norm()
+        at += n

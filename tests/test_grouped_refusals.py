@@ -176,3 +176,17 @@ def test_rotary_reference_turns_pairs(interleaved):
     got = rotary_reference(x, torch.tensor([math.pi / 2], dtype=torch.float64), torch.tensor(1),
                            interleaved)
     assert torch.allclose(got, torch.tensor([0.0, 1.0, 7.0]), atol=1e-6)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_reference_pairs_channels(interleaved):
+    # Three pairs turned by 90, 180 and 0 degrees, a channel behind them; by
+    # halves (0, 3) (1, 4) (2, 5), or neighbours.
+    freqs = torch.tensor([math.pi / 2, math.pi, 0.0], dtype=torch.float64)
+    x = torch.arange(1.0, 8.0, dtype=torch.float64)
+    want = ([-2.0, 1.0, -3.0, -4.0, 5.0, 6.0, 7.0] if interleaved
+            else [-4.0, -2.0, 3.0, 1.0, -5.0, 6.0, 7.0])
+    got = rotary_reference(x, freqs, torch.tensor(1), interleaved)
+    assert torch.allclose(got, torch.tensor(want, dtype=torch.float64), atol=1e-12)
+    doubled = rotary_reference(x, freqs, torch.tensor(1), interleaved, magnitude=2.0)
+    assert torch.allclose(doubled[:6], 2 * got[:6]) and doubled[6] == 7.0
