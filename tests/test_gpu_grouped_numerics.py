@@ -282,3 +282,29 @@ def test_rotary_then_attention_event_by_event(dtype, tol):
             else:
                 assert (a - b[0]).norm() <= tol * b.norm()
         at += n
+
+
+def test_fp16_powers_are_found_anew_on_every_replay():
+    # The powers of two that keep dS within fp16 come from the values of the
+    # replay, not of the capture.
+    lens = [300, 41]
+    leaves, g = _packed(lens, 4, 2, 64, FP16)
+    cu = _offsets(lens)
+    fixed = [torch.zeros_like(t) for t in (*leaves, g)]
+
+    def run(q, k, v, g):
+        q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+        return torch.autograd.grad(flash_grouped_attention_varlen(q, k, v, cu), (q, k, v), g)
+
+    run(*fixed)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run(*fixed)
+    for g_scale, v_scale in ((1.0, 1.0), (2.0**-10, 1.0), (2.0**9, 2.0**3), (2.0**-3, 2.0**-8)):
+        fresh = [leaves[0], leaves[1], leaves[2] * v_scale, g * g_scale]
+        with torch.no_grad():
+            for a, b in zip(fixed, fresh):
+                a.copy_(b)
+        graph.replay()
+        for a, b in zip(run(*fresh), outs):
+            assert torch.equal(a, b) and a.count_nonzero() > 0 and a.isfinite().all()
