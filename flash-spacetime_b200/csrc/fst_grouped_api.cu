@@ -55,6 +55,14 @@ bool any_null(std::initializer_list<const void*> ptrs) {
   return false;
 }
 
+// An address that is not a multiple of its element's size would fault on the GPU.
+bool misaligned(size_t size, std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if ((uintptr_t)p % size) return true;
+  return false;
+}
+size_t size_of(int dtype) { return dtype == FST_F32 ? 4 : 2; }
+
 int status(const char* where) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return api_fail(FST_ERR_CUDA, "%s: %s", where, cudaGetErrorString(e));
@@ -81,6 +89,10 @@ int check_rotary(const FstRotaryArgs& p) {
       return api_fail(FST_ERR_INVALID, "packed rows need cu_seqlens or positions");
     if (!p.q.data || !p.q_out.data || (p.k.data && !p.k_out.data) || (p.pairs > 0 && !p.freqs))
       return api_fail(FST_ERR_INVALID, "rotary: a required pointer is null");
+    if (misaligned(size_of(p.dtype), {p.q.data, p.k.data, p.q_out.data, p.k_out.data}) ||
+        misaligned(8, {p.freqs}) || misaligned(4, {p.cu_seqlens}) ||
+        misaligned(p.positions_64 ? 8 : 4, {p.positions}))
+      return api_fail(FST_ERR_INVALID, "rotary: a pointer is not aligned to its elements");
   }
   return FST_OK;
 }
@@ -96,6 +108,10 @@ int fst_grouped_forward(const FstGroupedForwardArgs* a, void* stream) {
   if (a->prob.total_rows == 0) return FST_OK;
   if (any_null({a->q.data, a->k.data, a->v.data, a->out.data, a->lse}))
     return api_fail(FST_ERR_INVALID, "grouped forward: q, k, v, out and lse are required");
+  if (misaligned(size_of(a->prob.dtype), {a->q.data, a->k.data, a->v.data, a->out.data,
+                                          a->out_low.data}) ||
+      misaligned(4, {a->lse, a->prob.seqlens, a->prob.cu_seqlens}))
+    return api_fail(FST_ERR_INVALID, "grouped forward: a pointer is not aligned to its elements");
   cudaGetLastError();  // clear a stale error so the check below is ours
   const cudaStream_t st = (cudaStream_t)stream;
   const int done = fst::grouped::tc_takes(*a) ? fst::grouped::tc_forward(*a, st)
@@ -111,6 +127,11 @@ int fst_grouped_backward(const FstGroupedBackwardArgs* a, void* stream) {
   if (any_null({a->q.data, a->k.data, a->v.data, a->out.data, a->dout.data, a->dq.data,
                 a->dk.data, a->dv.data, a->lse, a->stats}))
     return api_fail(FST_ERR_INVALID, "grouped backward: a required pointer is null");
+  if (misaligned(size_of(a->prob.dtype),
+                 {a->q.data, a->k.data, a->v.data, a->out.data, a->out_low.data, a->dout.data,
+                  a->dq.data, a->dk.data, a->dv.data}) ||
+      misaligned(4, {a->lse, a->stats, a->prob.seqlens, a->prob.cu_seqlens}))
+    return api_fail(FST_ERR_INVALID, "grouped backward: a pointer is not aligned to its elements");
   cudaGetLastError();
   const cudaStream_t st = (cudaStream_t)stream;
   const int done = fst::grouped::tc_takes(*a) ? fst::grouped::tc_backward(*a, st)

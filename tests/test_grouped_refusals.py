@@ -190,3 +190,53 @@ def test_rotary_reference_pairs_channels(interleaved):
     assert torch.allclose(got, torch.tensor(want, dtype=torch.float64), atol=1e-12)
     doubled = rotary_reference(x, freqs, torch.tensor(1), interleaved, magnitude=2.0)
     assert torch.allclose(doubled[:6], 2 * got[:6]) and doubled[6] == 7.0
+
+
+def _fill(a, size):
+    """Every pointer of an argument struct set to an address that is aligned to
+    ``size`` bytes; none is ever read."""
+    address = 4096 + size
+    for name, kind in a._fields_:
+        if kind is ctypes.c_void_p:
+            setattr(a, name, address)
+        elif kind is _lib.FstRows:
+            getattr(a, name).data = address
+    return a
+
+
+@pytest.mark.parametrize("dtype, size", [(_lib.FST_F32, 4), (_lib.FST_BF16, 2), (_lib.FST_F16, 2)])
+def test_misaligned_pointers_are_refused_before_a_launch(dtype, size):
+    lib = _lib.load()
+    before = lib.fst_kernel_launches()
+
+    def refused(entry, a):
+        assert entry(ctypes.byref(a), None) == _lib.FST_ERR_INVALID
+        assert "aligned" in _lib.last_error()
+
+    for entry, cls, names in (
+            (lib.fst_grouped_forward, _lib.FstGroupedForwardArgs,
+             ("q", "k", "v", "out", "out_low", "lse")),
+            (lib.fst_grouped_backward, _lib.FstGroupedBackwardArgs,
+             ("q", "k", "v", "out", "out_low", "dout", "dq", "dk", "dv", "lse", "stats"))):
+        for name in names:
+            a = _fill(cls(), 8)
+            a.prob = _grouped_args(dtype=dtype).prob
+            if isinstance(getattr(a, name), _lib.FstRows):
+                getattr(a, name).data += size // 2
+            else:
+                setattr(a, name, getattr(a, name) + 2)
+            refused(entry, a)
+        a = _fill(cls(), 8)
+        a.prob = _grouped_args(dtype=dtype, cu_seqlens=258).prob
+        refused(entry, a)
+    for name, off in (("q", size // 2), ("k_out", size // 2), ("freqs", 4), ("cu_seqlens", 2),
+                      ("positions", 4)):
+        a = _fill(_lib.FstRotaryArgs(), 8)
+        a.dtype, a.packed, a.batch, a.heads, a.kv_heads, a.head_dim, a.pairs = dtype, 1, 2, 4, 2, 32, 16
+        a.magnitude, a.total_rows, a.positions_64 = 1.0, 64, 1
+        if isinstance(getattr(a, name), _lib.FstRows):
+            getattr(a, name).data += off
+        else:
+            setattr(a, name, getattr(a, name) + off)
+        refused(lib.fst_rotary, a)
+    assert lib.fst_kernel_launches() == before
