@@ -308,3 +308,16 @@ def test_fp16_powers_are_found_anew_on_every_replay():
         graph.replay()
         for a, b in zip(run(*fresh), outs):
             assert torch.equal(a, b) and a.count_nonzero() > 0 and a.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 32), (FP16, 128), (FP32, 32)])
+def test_a_long_run_of_empty_events(dtype, dim):
+    # The work list gives every event a position, an empty one too.
+    leaves, g = _packed([200, 170], 2, 1, dim, dtype)
+    cu = torch.cat((torch.zeros(60000), torch.full((60000,), 200.0),
+                    torch.full((1000,), 370.0))).int().cuda()
+    out = flash_grouped_attention_varlen(*leaves, cu)
+    got = (out.detach(),) + torch.autograd.grad(out, leaves, g)
+    out = flash_grouped_attention_varlen(*leaves, _offsets([200, 170]))
+    want = (out.detach(),) + torch.autograd.grad(out, leaves, g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
