@@ -87,7 +87,13 @@ constexpr bool scaled() {
 }
 constexpr int kPBits = 14;  // P <= 1 of the column kernel times 2^14
 
-// Largest |dO| and |v| of a block's 128 rows of an event and key head (all
+// Magnitudes of two fp16 values; 0 for those that are not finite, which make
+// their own rows so whatever the powers, and must not shift those of others.
+__device__ __forceinline__ uint32_t magnitudes(uint32_t w) {
+  w &= 0x7fff7fff;
+  return w & __vcmpltu2(w, 0x7c007c00);
+}
+// Largest finite |dO| and |v| of a block's 128 rows of an event and key head (all
 // query heads of the group), as fp16 bits, low and high half of the word at the
 // block's first row in ranges[kv_heads][rows].
 __global__ void __launch_bounds__(256) range_kernel(const FstGroupedBackwardArgs a, int blocks,
@@ -100,8 +106,8 @@ __global__ void __launch_bounds__(256) range_kernel(const FstGroupedBackwardArgs
   auto largest = [&](const FstRows& x, int h, uint32_t m) {
     for (int e = threadIdx.x; e < n; e += 256) {
       const uint4 w = *(const uint4*)(row_ptr<__half>(x, t, h, t.i0 + e / vecs) + e % vecs * 8);
-      m = __vmaxu2(__vmaxu2(m, __vmaxu2(w.x & 0x7fff7fff, w.y & 0x7fff7fff)),
-                   __vmaxu2(w.z & 0x7fff7fff, w.w & 0x7fff7fff));
+      m = __vmaxu2(__vmaxu2(m, __vmaxu2(magnitudes(w.x), magnitudes(w.y))),
+                   __vmaxu2(magnitudes(w.z), magnitudes(w.w)));
     }
     return m;
   };
@@ -131,9 +137,9 @@ __device__ __forceinline__ uint32_t event_range(const uint32_t* ranges, const Fs
 __device__ __forceinline__ float half_bits(uint32_t x) {
   return __half2float(__ushort_as_half((unsigned short)x));
 }
-// Largest a for which 2^a 2 D g v stays below 2^15 (-26 to 62).
+// Largest a for which 2^a 2 D g v stays below 2^15 (-26 to 61).
 __device__ __forceinline__ int power_of(int D, float g, float v) {
-  const float bound = fminf(fmaxf(2.f * D * g * v, 0x1p-47f), 0x1p40f);
+  const float bound = fmaxf(2.f * D * g * v, 0x1p-47f);  // at most 2^40
   return 15 + 126 - (__float_as_int(bound) >> 23);  // bound < 2^((bits >> 23) - 126)
 }
 __device__ __forceinline__ float exp2i(int a) { return __int_as_float((a + 127) << 23); }
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         for (int e = 0; e < 4; ++e) {
           delta = fmaf(Elem<T>::lo(xs[e]) + Elem<T>::lo(zs[e]), Elem<T>::lo(ys[e]), delta);
           delta = fmaf(Elem<T>::hi(xs[e]) + Elem<T>::hi(zs[e]), Elem<T>::hi(ys[e]), delta);
-          if (scaled<T>()) peak = __vmaxu2(peak, ys[e] & 0x7fff7fff);
+          if (scaled<T>()) peak = __vmaxu2(peak, magnitudes(ys[e]));
         }
       }
     }

@@ -291,7 +291,8 @@ __device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, i
 #pragma unroll
   for (int c = 0; c < BRows / 16; ++c)
     if (c * 16 < rows)
-      mma_ts(d, P + c / 4 * 64 + c % 4 * 8 + (c == 2 || c == 3 ? gap : 0), x + c * XStep / 16, instr, add || c > 0, leader);
+      mma_ts(d, P + c / 4 * 64 + c % 4 * 8 + (c == 2 || c == 3 ? gap : 0), x + c * XStep / 16, instr,
+             add || c > 0, leader);
 }
 
 // The block's rows of no event: zeros, in 16-byte vectors, by n threads.

@@ -321,3 +321,25 @@ def test_a_long_run_of_empty_events(dtype, dim):
     out = flash_grouped_attention_varlen(*leaves, _offsets([200, 170]))
     want = (out.detach(),) + torch.autograd.grad(out, leaves, g)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype, dim", [(FP16, 64), (FP16, 128), (BF16, 64)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_gradient_row_that_is_not_finite_reaches_only_the_keys_it_sees(dtype, dim, value):
+    # (dq and dk: dv may meet it in a tile, as 0 * NaN.)
+    n, row = 500, 200
+    leaves, g = _packed([n], 4, 2, dim, dtype)
+    g *= 2.0**-6
+    cu = _offsets([n])
+
+    def run(x):
+        g[row] = x
+        out = flash_grouped_attention_varlen(*leaves, cu)
+        return torch.autograd.grad(out, leaves[:2], g)
+
+    for a, b, clean in zip(run(value), run(0.0), (slice(None), slice(row + 1, None))):
+        keep = torch.ones(n, dtype=torch.bool, device="cuda")
+        keep[row] = False
+        keep[:clean.start or 0] = False
+        assert torch.equal(a[keep], b[keep]) and a[keep].count_nonzero() > 0
+        assert not a[row].isfinite().all()
