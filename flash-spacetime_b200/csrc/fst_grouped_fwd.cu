@@ -10,13 +10,13 @@
 //            sum, writes P back over S as 16-bit values (the A operand of the
 //            second product), rescales O when the maximum has grown.
 //
-// Measured, bf16, 8192 rows, 16 heads, not causal: 487 us at Dh = 128 (1130
+// Measured, bf16, 8192 rows, 16 heads, not causal: 492 us at Dh = 128 (1117
 // TFLOP/s; the 64-wide Q K^T reads 4 KB of Q for every 2 KB of K, and O and
-// two S fill the 256 columns), 390 us at 64 and 382 us at 32, where the 2.7e12
-// exponentials a second are 60 % of the unit's 16 a cycle and SM: the rest is
+// two S fill the 256 columns), 414 us at 64 and 392 us at 32, where the 2.6e12
+// exponentials a second are 57 % of the unit's 16 a cycle and SM: the rest is
 // the chain from one tile's S to its P (load 200 cycles, maximum 100, vote 90,
 // exponentials 770, stores and barriers 200). Tiles whose keys all rows see
-// run without masks (16384 causal of 64: 540 -> 470 us).
+// run without masks (16384 causal of 64: 540 -> 470 us when that came in).
 //
 // Softmax in the base-2 domain: p = 2^(c s - c m), c = |scale| log2(e) (the
 // sign of the scale is the product's own negate bit). O and l are rescaled

@@ -30,9 +30,11 @@ namespace fst {
 namespace {
 
 constexpr int kThreads = 256;
-// Measured at [21020, 32 + 8, 128] bf16 with 2 heads in flight and 10 heads a
-// thread, four blocks an SM: 79 us, 5.4 TB/s (4 in flight and 4 a thread,
-// three blocks: 91 us; 1 and 10, six blocks: 98 us).
+// Measured at [21020, 32 + 8, 128] bf16, half layout, with 2 heads in flight and
+// 10 heads a thread, four blocks an SM: 77 us, 5.6 TB/s (4 in flight and 4 a
+// thread, three blocks: 91 us; 1 and 10, six blocks: 98 us). Chosen on that
+// shape alone; at four blocks' 64 registers the vector variants spill some
+// (16-bit 32 bytes, fp32 16), and interleaved 16-bit rows run at 3.9 TB/s.
 constexpr int kHeads = 2;         // heads of a thread in flight
 constexpr int kWalk = 10;         // heads of a thread
 constexpr int kMaxRows = 32;      // rows per block

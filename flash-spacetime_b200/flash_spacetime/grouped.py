@@ -17,8 +17,15 @@ Conventions:
   to run (no atomics);
 * with gradients, a 16-bit forward also keeps what rounding its output left
   over, so that the backward's row sums ``D = dO . out`` are those of the
-  unrounded output: rows of few keys would otherwise carry its rounding into
-  dq and dk;
+  unrounded output: dq and dk would otherwise carry its rounding, times any
+  offset that the values share;
+* a row that sees one key (the row of an event of one, row 0 of a causal event)
+  has a dq, and a share in dk, of exactly 0;
+* fp16 gradients keep their small values whatever the gradient's scale: dS
+  carries powers of two taken from the event's largest finite values;
+* calls without a gradient launch directly, unless a trace is being recorded or
+  a forward-mode level or ``torch.func`` transform is active, which the autograd
+  node runs or refuses;
 * inputs are read in place whatever their strides, as long as the channels of
   a head are adjacent: slices of a fused projection need no copy;
 * forward and backward may be captured into CUDA graphs (lengths on the device;

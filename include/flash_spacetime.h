@@ -290,7 +290,8 @@ typedef struct FstGroupedBackwardArgs {
   FstRows v;
   FstRows out;           /* forward output                                   */
   FstRows out_low;       /* forward output or data NULL: with it D_i = dout_i . */
-                         /* out_i keeps the rows of few keys exact           */
+                         /* out_i is that of out before its rounding, which  */
+                         /* would go into dq and dk                          */
   FstRows dout;          /* its gradient; padding rows ignored               */
   FstRows dq;            /* outputs                                          */
   FstRows dk;
