@@ -41,12 +41,6 @@
 // at Dh = 128; 430 and 650 us at 64; 412 and 598 us at 32. At 128 the tensor
 // cores are busy half the time, at 64 the exponentials' unit; what remains is
 // the chain of a tile's steps.
-//
-// dS is rounded once to the type for its product (twice where a row sees few
-// keys, below). Its sum over a row's keys is 0 before the rounding and not after,
-// so an offset c that all keys share reaches dq as c times that: keys of mean 2
-// (8) and deviation 1 leave dq of 256 keys off by 3 (11) times one rounding of it,
-// where keys of mean 0 leave 1.45.
 
 #include <cuda_runtime.h>
 
@@ -152,16 +146,38 @@ __device__ __forceinline__ float exp2i(int a) { return __int_as_float((a + 127) 
 
 // ---- dq ---------------------------------------------------------------------
 
+// The sum of dS over a row's keys is 0 before the rounding to 16 bits (and but
+// for that of D) and not after, and an offset that all keys share would reach dq
+// times that: keys of mean 2 (8) and deviation 1 left dq of 256 keys off by 3 (11)
+// times one rounding of it, keys of mean 0 by 1.45. So a row c is taken off all
+// keys, which changes nothing but that: the mean of the event's first 16, rounded
+// to the type (then 1.45 for all three).
+// One group: the product dS K is followed by dS times rows of -c, for which c has
+// to be there by the first tile's dS (dq of 256 short events 261 -> 281 us, of
+// 16384 causal of 64 522 -> 538; the second way takes 295 and 526).
+struct RowsOne {
+  alignas(1024) uint32_t less[16 * 32];  // 16 rows of -c, as a tile
+};
+// Two groups: dS times ones sums the rows up, and the sum times c is taken off
+// when the result is stored (documents of 128: 187 -> 193 us; 8192 rows of 16 heads
+// 738 -> 765). Tensor cores have less time to spare there, and shared memory no
+// room: 1 KB more than this would take the next larger share of L1 (201 us).
+struct RowsTwo {
+  float delta[2][kBM];  // the groups' shares of D
+  union {               // the first until all have read it
+    uint16_t peak[2][kBM];  // and of max|dO| (fp16)
+    Ones ones;
+  };
+  alignas(16) uint32_t c[64];
+};
 template <int Boxes, int W, int Stages>
 struct RowSmem {
   alignas(1024) char q[Boxes * kBM * 128];
   alignas(1024) char g[Boxes * kBM * 128];
   alignas(1024) char k[Stages][Boxes * W * 64 * 128];
   alignas(1024) char v[Stages][Boxes * W * 64 * 128];
-  float delta[2][kBM];    // the groups' shares of D
-  uint16_t peak[2][kBM];  // and of max|dO| (fp16). At two groups 1 KB more than this would
-                          // take the next larger share of L1 (dq of documents 186 -> 201 us)
-  uint64_t own_full, full[Stages], empty[Stages], s_full, s_free, dp_full, ds_ready, done;
+  typename std::conditional<W == 1, RowsOne, RowsTwo>::type more;
+  uint64_t own_full, full[Stages], empty[Stages], s_full, s_free, dp_full, ds_ready, c_full, done;
   uint32_t tmem;
 };
 
@@ -185,6 +201,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     mbar_init(smem_addr(&sm.s_free), W * 4);
     mbar_init(smem_addr(&sm.dp_full), 1);
     mbar_init(smem_addr(&sm.ds_ready), W * 4);
+    mbar_init(smem_addr(&sm.c_full), 1);
     mbar_init(smem_addr(&sm.done), 1);
     mbar_init_fence();
     prefetch_map(&maps.q);
@@ -221,11 +238,38 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem;  // S, dP (dS over it), dQ
+  const uint32_t tmem = sm.tmem;  // S, dP (dS over it), dQ, with two groups sums of dS
 
   bool ok = true;
   if (warp == kTma) {
+    // Meanwhile c, two channels of each box a lane. (From the first tile: this
+    // warp alone brings the next one into its place.)
+    const int rows = min(t.len, 16);
+    const float each = __fdividef(1.f, (float)rows);
+    ok = mbar_wait(smem_addr(&sm.full[0]), 0);
+#pragma unroll
+    for (int b = 0; b < Boxes; ++b) {
+      float x = 0.f, y = 0.f;
+#pragma unroll 8
+      for (int j = 0; j < rows; ++j) {
+        const uint32_t w = *(const uint32_t*)(sm.k[0] + b * kBN * 128 + j * 128 +
+                                              ((lane / 4) ^ (j & 7)) * 16 + lane % 4 * 4);
+        x += Elem<T>::lo(w);
+        y += Elem<T>::hi(w);
+      }
+      if constexpr (W == 1) {
+        const uint32_t less = Elem<T>::pack(-x * each, -y * each);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          sm.more.less[j * 32 + ((lane / 4) ^ (j & 7)) * 4 + lane % 4] = less;
+        fence_proxy_async();
+      } else {
+        sm.more.c[b * 32 + lane] = Elem<T>::pack(x * each, y * each);
+      }
+    }
+    __syncwarp();
     if (lane == 0) {
+      mbar_arrive(smem_addr(&sm.c_full));
       for (int it = Stages; it < tiles && ok; ++it) {
         ok = mbar_wait(smem_addr(&sm.empty[it % Stages]), (it / Stages - 1) & 1);
         if (ok) load(it);
@@ -234,7 +278,8 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
   } else if (warp == kMma) {
     const uint32_t leader = elect_one();
     const int n = uniform(tiles), last = uniform(end), dim = uniform(D);
-    const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, q_mem = p_mem + kBN;
+    const uint32_t s_mem = uniform(tmem), p_mem = s_mem + kBN, q_mem = p_mem + kBN,
+                   sum_mem = q_mem + Boxes * 64;
     const uint32_t acc_instr = instruction<T>((dim + 15) & ~15, true, false);
     const bool few = uniform(few_keys(p, t));
     auto keys = [&](int it) { return min(kBN, last - it * kBN); };
@@ -251,6 +296,22 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
                                   (keys(it) + 15) & ~15, false, leader);
       tc_commit(smem_addr(&sm.dp_full), leader);
     };
+    // (fp16: when the groups have read what lies there.)
+    constexpr bool kLate = W == 2 && scaled<T>();
+    auto ready = [&] {
+      if constexpr (W == 2) {
+        fill_ones<T>(sm.more.ones, lane);
+        __syncwarp();
+      }
+    };
+    // dS of a tile, or its second part, times -c or ones.
+    auto correct = [&](uint32_t dS, int rows, bool add, uint32_t gap) {
+      if constexpr (W == 1)
+        accumulate<kBN, 0>(q_mem, dS, smem_addr(sm.more.less), rows, acc_instr, true, leader, gap);
+      else
+        row_sums<T, kBN>(sum_mem, dS, smem_addr(&sm.more.ones), rows, add, leader, gap);
+    };
+    if (!kLate) ready();  // while the first tiles are on their way
     ok = mbar_wait(smem_addr(&sm.own_full), 0) && logits(0);
     if (ok) weights(0);
     for (int it = 0; it < n && ok; ++it) {
@@ -262,12 +323,19 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       ok = ok && mbar_wait(smem_addr(&sm.ds_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
+      if (kLate && it == 0) ready();
       const bool second = few && it == 0;
       accumulate<kBN>(q_mem, p_mem, smem_addr(sm.k[it % Stages]), keys(it), acc_instr, it > 0,
                       leader, second ? kFewGap : 0);
       if (second)
         accumulate<kBN>(q_mem, p_mem + kFewGap, smem_addr(sm.k[0]), min(last, kFew), acc_instr,
                         true, leader);
+      if (W == 1 && it == 0) {
+        ok = mbar_wait(smem_addr(&sm.c_full), 0);
+        if (!ok) break;
+      }
+      correct(p_mem, keys(it), it > 0, second ? kFewGap : 0);
+      if (second) correct(p_mem + kFewGap, min(last, kFew), true, 0);
       tc_commit(smem_addr(&sm.empty[it % Stages]), leader);
       if (it + 1 < n) weights(it + 1);
     }
@@ -302,12 +370,12 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         }
       }
     }
-    if (W == 2) {
-      sm.delta[w][row] = delta;
-      if (scaled<T>()) sm.peak[w][row] = (uint16_t)max(peak & 0xffff, peak >> 16);
+    if constexpr (W == 2) {
+      sm.more.delta[w][row] = delta;
+      if (scaled<T>()) sm.more.peak[w][row] = (uint16_t)max(peak & 0xffff, peak >> 16);
       tc::named_sync(1, W * 128);
-      delta = sm.delta[0][row] + sm.delta[1][row];
-      if (scaled<T>()) peak = max(sm.peak[0][row], sm.peak[1][row]);
+      delta = sm.more.delta[0][row] + sm.more.delta[1][row];
+      if (scaled<T>()) peak = max(sm.more.peak[0][row], sm.more.peak[1][row]);
     }
     if (live) {
       const int64_t st = stat_at(p, t, p.heads, at.h, i);
@@ -400,9 +468,16 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
     // The groups share the columns of the result.
-    store_row<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr,
-                 tmem + quad + 2 * kBN + w * 64, W == 1 ? D : min(D - w * 64, 64),
-                 ok ? undo : NAN);
+    T* dst = live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr;
+    const uint32_t acc = tmem + quad + 2 * kBN + w * 64;
+    if constexpr (W == 1) {
+      store_row<T>(dst, acc, D, ok ? undo : NAN);
+    } else {
+      ok = ok && mbar_wait(smem_addr(&sm.c_full), 0);
+      store_row<T, false, false, true>(dst, acc, min(D - w * 64, 64), ok ? undo : NAN, nullptr,
+                                       (const T*)sm.more.c + w * 64,
+                                       tmem + quad + 2 * kBN + Boxes * 64);
+    }
     tc_fence_before();
   }
   __syncthreads();

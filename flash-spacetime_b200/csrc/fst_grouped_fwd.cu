@@ -53,7 +53,7 @@ struct FwdSmem {
   alignas(1024) char q[Boxes * kBM * 128];
   alignas(1024) char k[Stages][Boxes * kBN * 128];
   alignas(1024) char v[Stages][Boxes * kBN * 128];
-  alignas(1024) uint4 ones[Boxes == 1 ? 16 * 8 : 1];  // 16 rows of 64 channels of 1
+  Ones ones;
   Feed feed;
   uint64_t q_full, q_empty, o_free;
   uint64_t k_full[Stages], k_empty[Stages], v_full[Stages], v_empty[Stages];
@@ -99,11 +99,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     prefetch_map(&maps.k);
     prefetch_map(&maps.v);
   }
-  if (kOnes && threadIdx.x < 128) {
-    const uint32_t one = Elem<T>::pack(1.f, 1.f);
-    sm.ones[threadIdx.x] = make_uint4(one, one, one, one);
-    fence_proxy_async();
-  }
+  if (kOnes && warp == 0) fill_ones<T>(sm.ones, lane);
   if (warp == 5) tmem_alloc<kCols>(smem_addr(&sm.tmem));
   tc_fence_before();
   __syncthreads();
@@ -212,8 +208,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         accumulate<kBN>(o_mem, s_mem + g % 2 * kBN, smem_addr(sm.v[s]), keys(it), o_instr, it > 0,
                         leader);
         if (kOnes)
-          accumulate<kBN, 0>(o_mem + 64, s_mem + g % 2 * kBN, smem_addr(sm.ones), keys(it),
-                             instruction<T>(16, true, false), it > 0, leader);
+          row_sums<T, kBN>(o_mem + 64, s_mem + g % 2 * kBN, smem_addr(&sm.ones), keys(it), it > 0,
+                           leader);
         tc_commit(smem_addr(&sm.pv_done[g % 2]), leader);
         tc_commit(smem_addr(&sm.v_empty[s]), leader);
         if (it + 2 < tiles) ok = logits(it + 2);
@@ -334,7 +330,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       T* out = seen ? (T*)a.out.data + item.out_at + row * a.out.row_stride : nullptr;
       if (ok) ok = mbar_wait(smem_addr(&sm.pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1);
       tc_fence_after();
-      if (kOnes) l_used = tmem_ld1(tO + quad + 64);
+      if (kOnes) {
+        l_used = tmem_ld1(tO + quad + 64);
+        tmem_wait_ld();
+        pin(l_used);
+      }
       const float f = ok ? 1.f / l_used : NAN;
       T* low = Low && seen ? row_ptr<T>(a.out_low, t, item.h, i) : nullptr;
       if (Low && Boxes == 1) {

@@ -145,17 +145,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&x)[16]
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-// One column, waited for.
+// One column; may be used after tmem_wait_ld(), and a pin.
 __device__ __forceinline__ float tmem_ld1(uint32_t addr) {
   float x;
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(x)
-      : "r"(addr)
-      : "memory");
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(x) : "r"(addr) : "memory");
   return x;
 }
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+f"(x)); }
 // 16 columns in place: each row times its factor. Waits for itself.
 __device__ __forceinline__ void tmem_scale16(uint32_t addr, float f) {
   uint32_t x[16];
@@ -294,6 +290,30 @@ __device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, i
       mma_ts(d, P + c / 4 * 64 + c % 4 * 8 + (c == 2 || c == 3 ? gap : 0), x + c * XStep / 16, instr,
              add || c > 0, leader);
 }
+// d[128][16] (+)= the row sums of P over `rows` columns, the same in all 16: a
+// product with 16 x 16 ones, 512 bytes of them at `ones` (no swizzle: 128-byte
+// blocks of 8 x 8, their order of no matter). As rounded for the product beside it.
+struct Ones {
+  alignas(128) uint4 x[32];
+};
+template <typename T>
+__device__ __forceinline__ void fill_ones(Ones& ones, int t) {  // threads 0 to 31
+  const uint32_t one = Elem<T>::pack(1.f, 1.f);
+  ones.x[t] = make_uint4(one, one, one, one);
+  fence_proxy_async();
+}
+template <typename T, int BRows>
+__device__ __forceinline__ void row_sums(uint32_t d, uint32_t P, uint32_t ones, int rows, bool add,
+                                         uint32_t leader, uint32_t gap = 0) {
+  const uint64_t x = (uint64_t)((ones >> 4) & 0x3fff) | (uint64_t)(128 >> 4) << 16 |
+                     (uint64_t)(256 >> 4) << 32 | (uint64_t)1 << 46;
+  const uint32_t instr = instruction<T>(16, false, false);
+#pragma unroll
+  for (int c = 0; c < BRows / 16; ++c)
+    if (c * 16 < rows)
+      mma_ts(d, P + c / 4 * 64 + c % 4 * 8 + (c == 2 || c == 3 ? gap : 0), x, instr, add || c > 0,
+             leader);
+}
 
 // The block's rows of no event: zeros, in 16-byte vectors, by n threads.
 template <typename T, int BM>
@@ -322,17 +342,34 @@ __device__ __forceinline__ void store16(void* dst, const uint32_t (&w)[8]) {
 // A thread's row of D accumulator columns, times f, rounded and stored (whole
 // warps; out may be null). `Low`: what that rounding leaves over, instead;
 // `Both`: that too, to `low` (may be null), in one pass over the accumulator.
-template <typename T, bool Low = false, bool Both = false>
-__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f,
-                                          T* low = nullptr) {
+// `Shift`: less the row `mean` (16-bit values in shared memory) times the value
+// in column `sum_at`.
+template <typename T, bool Low = false, bool Both = false, bool Shift = false>
+__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f, T* low = nullptr,
+                                          const T* mean = nullptr, uint32_t sum_at = 0) {
+  float sum = 0.f;
+  if (Shift) sum = tmem_ld1(sum_at);
   for (int d = 0; d < D; d += 32) {
     float o[32];
     tmem_ld32(o, acc + d);
     tmem_wait_ld();
     pin(o);
+    if (Shift && d == 0) pin(sum);
 #pragma unroll
     for (int e = 0; e < 32; e += 16) {
       if (!out || d + e >= D) break;
+      if (Shift) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+          const uint4 c = *(const uint4*)(mean + d + e + i);
+          const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            o[e + i + 2 * u] = fmaf(-sum, Elem<T>::lo(cs[u]), o[e + i + 2 * u]);
+            o[e + i + 2 * u + 1] = fmaf(-sum, Elem<T>::hi(cs[u]), o[e + i + 2 * u + 1]);
+          }
+        }
+      }
       auto put = [&](T* dst, const uint32_t (&w)[8]) {
         if (d + e + 16 <= D)
           store16(dst + d + e, w);

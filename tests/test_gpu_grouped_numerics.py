@@ -105,7 +105,7 @@ def _definition(q, k, v, g, causal, scale):
 
 
 def _roundings(events, n, heads, kv_heads, dim, dtype, causal, v_mean=0.0, g_mean=0.0,
-               g_scale=1.0, rows=slice(None), seed=0):
+               g_scale=1.0, rows=slice(None), seed=0, k_mean=0.0):
     """Root mean square error of each result over that of rounding it once."""
     gen = torch.Generator(device="cuda").manual_seed(seed)
 
@@ -113,7 +113,7 @@ def _roundings(events, n, heads, kv_heads, dim, dtype, causal, v_mean=0.0, g_mea
         t = torch.randn(events * n, h, dim, device="cuda", generator=gen)
         return (scale * (t + mean)).to(dtype)
 
-    q, k, v = (t.requires_grad_(True) for t in (rand(heads), rand(kv_heads),
+    q, k, v = (t.requires_grad_(True) for t in (rand(heads), rand(kv_heads, k_mean),
                                                 rand(kv_heads, v_mean)))
     g = rand(heads, g_mean, g_scale)
     out = flash_grouped_attention_varlen(q, k, v, _offsets([n] * events), causal=causal)
@@ -343,3 +343,16 @@ def test_a_gradient_row_that_is_not_finite_reaches_only_the_keys_it_sees(dtype, 
         keep[:clean.start or 0] = False
         assert torch.equal(a[keep], b[keep]) and a[keep].count_nonzero() > 0
         assert not a[row].isfinite().all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (FP16, 64), (BF16, 128), (FP16, 72), (BF16, 24)])
+@pytest.mark.parametrize("mean", [2.0, 8.0])
+def test_a_common_offset_of_k_leaves_the_gradients_alone(dtype, dim, causal, mean):
+    # dS sums to 0 over a row's keys but for its rounding, and what that leaves
+    # times the offset is taken off dq again. Model: 1.1 for three keys (5.6 with
+    # a mean of 8 left in), 1.5 for 256 (11).
+    few = _roundings(300, 3, 4, 2, dim, dtype, causal, k_mean=mean)
+    assert few["dq"] <= 1.3 and few["dk"] <= 1.3, few
+    more = _roundings(8, 256, 4, 2, dim, dtype, causal, k_mean=mean)
+    assert more["dq"] <= 1.7 and more["dk"] <= 1.7, more
