@@ -37,8 +37,8 @@
 // whose products are 128 wide: a product of two shared-memory operands reads
 // 4 KB of A per 16 channels whatever its width, which bounds 64 wide ones.
 //
-// Measured, bf16, 8192 rows, 16 heads, not causal: rows 734 us, columns 801 us
-// at Dh = 128; 430 and 650 us at 64; 412 and 598 us at 32. At 128 the tensor
+// Measured, bf16, 8192 rows, 16 heads, not causal: rows 765 us, columns 805 us
+// at Dh = 128; 440 and 648 us at 64; 425 and 599 us at 32. At 128 the tensor
 // cores are busy half the time, at 64 the exponentials' unit; what remains is
 // the chain of a tile's steps.
 
@@ -152,31 +152,26 @@ __device__ __forceinline__ float exp2i(int a) { return __int_as_float((a + 127) 
 // times one rounding of it, keys of mean 0 by 1.45. So a row c is taken off all
 // keys, which changes nothing but that: the mean of the event's first 16, rounded
 // to the type (then 1.45 for all three).
-// One group: the product dS K is followed by dS times rows of -c, for which c has
-// to be there by the first tile's dS (dq of 256 short events 261 -> 281 us, of
-// 16384 causal of 64 522 -> 538; the second way takes 295 and 526).
-struct RowsOne {
-  alignas(1024) uint32_t less[16 * 32];  // 16 rows of -c, as a tile
-};
-// Two groups: dS times ones sums the rows up, and the sum times c is taken off
-// when the result is stored (documents of 128: 187 -> 193 us; 8192 rows of 16 heads
-// 738 -> 765). Tensor cores have less time to spare there, and shared memory no
-// room: 1 KB more than this would take the next larger share of L1 (201 us).
-struct RowsTwo {
-  float delta[2][kBM];  // the groups' shares of D
-  union {               // the first until all have read it
-    uint16_t peak[2][kBM];  // and of max|dO| (fp16)
-    Ones ones;
-  };
-  alignas(16) uint32_t c[64];
-};
+// A product of dS with ones sums the rows up, and the sum times c is taken off when
+// the result is stored (dq of 256 short events 261 -> 285 us, 16384 causal of 64
+// 522 -> 530, documents of 128 187 -> 192, 8192 rows of 16 heads 738 -> 765). c in
+// registers by the time the products end: read from shared memory then, 302 for the
+// short events. A product of dS with rows of -c in place of the sums: 281, and 534 for
+// the long one, whose pass at the power limit takes 2 % more.
 template <int Boxes, int W, int Stages>
 struct RowSmem {
   alignas(1024) char q[Boxes * kBM * 128];
   alignas(1024) char g[Boxes * kBM * 128];
   alignas(1024) char k[Stages][Boxes * W * 64 * 128];
   alignas(1024) char v[Stages][Boxes * W * 64 * 128];
-  typename std::conditional<W == 1, RowsOne, RowsTwo>::type more;
+  // At two groups 1 KB more than this would take the next larger share of L1 (dq of
+  // documents 187 -> 201 us).
+  float delta[2][kBM];  // the groups' shares of D
+  union {               // the first until all have read it
+    uint16_t peak[2][kBM];  // and of max|dO| (fp16)
+    Ones ones;
+  };
+  alignas(16) uint32_t c[Boxes * 32];
   uint64_t own_full, full[Stages], empty[Stages], s_full, s_free, dp_full, ds_ready, c_full, done;
   uint32_t tmem;
 };
@@ -189,6 +184,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
   extern __shared__ char raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   constexpr int kBN = W * 64, kCols = W * 256, kTma = W * 4, kMma = kTma + 1;
+  static_assert(W == 1 || sizeof(Smem) + 2048 <= 196 * 1024, "leaves L1 its share (RowSmem)");
   const FstGroupedProblem& p = a.prob;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == kTma && lane == 0) {
@@ -238,7 +234,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem;  // S, dP (dS over it), dQ, with two groups sums of dS
+  const uint32_t tmem = sm.tmem;  // S, dP (dS over it), dQ, sums of dS
 
   bool ok = true;
   if (warp == kTma) {
@@ -257,15 +253,7 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         x += Elem<T>::lo(w);
         y += Elem<T>::hi(w);
       }
-      if constexpr (W == 1) {
-        const uint32_t less = Elem<T>::pack(-x * each, -y * each);
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          sm.more.less[j * 32 + ((lane / 4) ^ (j & 7)) * 4 + lane % 4] = less;
-        fence_proxy_async();
-      } else {
-        sm.more.c[b * 32 + lane] = Elem<T>::pack(x * each, y * each);
-      }
+      sm.c[b * 32 + lane] = Elem<T>::pack(x * each, y * each);
     }
     __syncwarp();
     if (lane == 0) {
@@ -296,22 +284,13 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
                                   (keys(it) + 15) & ~15, false, leader);
       tc_commit(smem_addr(&sm.dp_full), leader);
     };
-    // (fp16: when the groups have read what lies there.)
+    // The ones, while the first tiles are on their way, or when the groups have read
+    // what lies there.
     constexpr bool kLate = W == 2 && scaled<T>();
-    auto ready = [&] {
-      if constexpr (W == 2) {
-        fill_ones<T>(sm.more.ones, lane);
-        __syncwarp();
-      }
-    };
-    // dS of a tile, or its second part, times -c or ones.
-    auto correct = [&](uint32_t dS, int rows, bool add, uint32_t gap) {
-      if constexpr (W == 1)
-        accumulate<kBN, 0>(q_mem, dS, smem_addr(sm.more.less), rows, acc_instr, true, leader, gap);
-      else
-        row_sums<T, kBN>(sum_mem, dS, smem_addr(&sm.more.ones), rows, add, leader, gap);
-    };
-    if (!kLate) ready();  // while the first tiles are on their way
+    if (!kLate) {
+      fill_ones<T>(sm.ones, lane);
+      __syncwarp();
+    }
     ok = mbar_wait(smem_addr(&sm.own_full), 0) && logits(0);
     if (ok) weights(0);
     for (int it = 0; it < n && ok; ++it) {
@@ -323,19 +302,21 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
       ok = ok && mbar_wait(smem_addr(&sm.ds_ready), it & 1);
       if (!ok) break;
       tc_fence_after();
-      if (kLate && it == 0) ready();
+      if (kLate && it == 0) {
+        fill_ones<T>(sm.ones, lane);
+        __syncwarp();
+      }
       const bool second = few && it == 0;
       accumulate<kBN>(q_mem, p_mem, smem_addr(sm.k[it % Stages]), keys(it), acc_instr, it > 0,
                       leader, second ? kFewGap : 0);
-      if (second)
+      row_sums<T, kBN>(sum_mem, p_mem, smem_addr(&sm.ones), keys(it), it > 0, leader,
+                       second ? kFewGap : 0);
+      if (second) {
         accumulate<kBN>(q_mem, p_mem + kFewGap, smem_addr(sm.k[0]), min(last, kFew), acc_instr,
                         true, leader);
-      if (W == 1 && it == 0) {
-        ok = mbar_wait(smem_addr(&sm.c_full), 0);
-        if (!ok) break;
+        row_sums<T, kBN>(sum_mem, p_mem + kFewGap, smem_addr(&sm.ones), min(last, kFew), true,
+                         leader);
       }
-      correct(p_mem, keys(it), it > 0, second ? kFewGap : 0);
-      if (second) correct(p_mem + kFewGap, min(last, kFew), true, 0);
       tc_commit(smem_addr(&sm.empty[it % Stages]), leader);
       if (it + 1 < n) weights(it + 1);
     }
@@ -370,12 +351,12 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
         }
       }
     }
-    if constexpr (W == 2) {
-      sm.more.delta[w][row] = delta;
-      if (scaled<T>()) sm.more.peak[w][row] = (uint16_t)max(peak & 0xffff, peak >> 16);
+    if (W == 2) {
+      sm.delta[w][row] = delta;
+      if (scaled<T>()) sm.peak[w][row] = (uint16_t)max(peak & 0xffff, peak >> 16);
       tc::named_sync(1, W * 128);
-      delta = sm.more.delta[0][row] + sm.more.delta[1][row];
-      if (scaled<T>()) peak = max(sm.more.peak[0][row], sm.more.peak[1][row]);
+      delta = sm.delta[0][row] + sm.delta[1][row];
+      if (scaled<T>()) peak = max(sm.peak[0][row], sm.peak[1][row]);
     }
     if (live) {
       const int64_t st = stat_at(p, t, p.heads, at.h, i);
@@ -465,19 +446,22 @@ __global__ void __launch_bounds__(threads_of(W), resident_of(W))
     for (; it < whole && ok; ++it) ok = tile(std::true_type(), std::false_type(), it);
     if (few_keys(p, t)) ok = tile(std::false_type(), std::true_type(), it++);
     for (; it < tiles && ok; ++it) ok = tile(std::false_type(), std::false_type(), it);
-    if (ok) ok = mbar_wait(smem_addr(&sm.done), 0);
+    uint32_t c[32];
+    ok = ok && mbar_wait(smem_addr(&sm.c_full), 0);
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      const uint4 x = *(const uint4*)(sm.c + w * 32 + e);
+      c[e] = x.x;
+      c[e + 1] = x.y;
+      c[e + 2] = x.z;
+      c[e + 3] = x.w;
+    }
+    ok = ok && mbar_wait(smem_addr(&sm.done), 0);
     tc_fence_after();
     // The groups share the columns of the result.
-    T* dst = live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr;
-    const uint32_t acc = tmem + quad + 2 * kBN + w * 64;
-    if constexpr (W == 1) {
-      store_row<T>(dst, acc, D, ok ? undo : NAN);
-    } else {
-      ok = ok && mbar_wait(smem_addr(&sm.c_full), 0);
-      store_row<T, false, false, true>(dst, acc, min(D - w * 64, 64), ok ? undo : NAN, nullptr,
-                                       (const T*)sm.more.c + w * 64,
-                                       tmem + quad + 2 * kBN + Boxes * 64);
-    }
+    store_row_less<T>(live ? row_ptr<T>(a.dq, t, at.h, i) + w * 64 : nullptr,
+                      tmem + quad + 2 * kBN + w * 64, W == 1 ? D : min(D - w * 64, 64),
+                      ok ? undo : NAN, c, tmem + quad + 2 * kBN + Boxes * 64);
     tc_fence_before();
   }
   __syncthreads();

@@ -278,8 +278,8 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t A, uint32_t B, int 
 // d[128][n] (+)= P X over `rows` rows (rounded up to 16) of X, a tile of BRows
 // rows; P 16-bit values in tensor memory, 64 rows of X in 32 columns, the
 // next 64 from 64 columns on; `gap` columns between the first 32 rows' and the
-// next 32's. XStep: bytes of 16 rows of X (0: the same rows every time).
-template <int BRows, int XStep = 2048>
+// next 32's.
+template <int BRows>
 __device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, int rows,
                                            uint32_t instr, bool add, uint32_t leader,
                                            uint32_t gap = 0) {
@@ -287,7 +287,7 @@ __device__ __forceinline__ void accumulate(uint32_t d, uint32_t P, uint32_t X, i
 #pragma unroll
   for (int c = 0; c < BRows / 16; ++c)
     if (c * 16 < rows)
-      mma_ts(d, P + c / 4 * 64 + c % 4 * 8 + (c == 2 || c == 3 ? gap : 0), x + c * XStep / 16, instr,
+      mma_ts(d, P + c / 4 * 64 + c % 4 * 8 + (c == 2 || c == 3 ? gap : 0), x + c * 2048 / 16, instr,
              add || c > 0, leader);
 }
 // d[128][16] (+)= the row sums of P over `rows` columns, the same in all 16: a
@@ -342,34 +342,17 @@ __device__ __forceinline__ void store16(void* dst, const uint32_t (&w)[8]) {
 // A thread's row of D accumulator columns, times f, rounded and stored (whole
 // warps; out may be null). `Low`: what that rounding leaves over, instead;
 // `Both`: that too, to `low` (may be null), in one pass over the accumulator.
-// `Shift`: less the row `mean` (16-bit values in shared memory) times the value
-// in column `sum_at`.
-template <typename T, bool Low = false, bool Both = false, bool Shift = false>
-__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f, T* low = nullptr,
-                                          const T* mean = nullptr, uint32_t sum_at = 0) {
-  float sum = 0.f;
-  if (Shift) sum = tmem_ld1(sum_at);
+template <typename T, bool Low = false, bool Both = false>
+__device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f,
+                                          T* low = nullptr) {
   for (int d = 0; d < D; d += 32) {
     float o[32];
     tmem_ld32(o, acc + d);
     tmem_wait_ld();
     pin(o);
-    if (Shift && d == 0) pin(sum);
 #pragma unroll
     for (int e = 0; e < 32; e += 16) {
       if (!out || d + e >= D) break;
-      if (Shift) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 8) {
-          const uint4 c = *(const uint4*)(mean + d + e + i);
-          const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            o[e + i + 2 * u] = fmaf(-sum, Elem<T>::lo(cs[u]), o[e + i + 2 * u]);
-            o[e + i + 2 * u + 1] = fmaf(-sum, Elem<T>::hi(cs[u]), o[e + i + 2 * u + 1]);
-          }
-        }
-      }
       auto put = [&](T* dst, const uint32_t (&w)[8]) {
         if (d + e + 16 <= D)
           store16(dst + d + e, w);
@@ -387,6 +370,39 @@ __device__ __forceinline__ void store_row(T* out, uint32_t acc, int D, float f, 
       if (Both && low) put(low, r);
     }
     __syncwarp();  // tcgen05.ld takes the whole warp
+  }
+}
+
+// The same of up to 64 columns, less the row c (16-bit pairs, held in registers from
+// before the accumulator is done) times the value in column `sum_at`.
+template <typename T>
+__device__ __forceinline__ void store_row_less(T* out, uint32_t acc, int D, float f,
+                                               const uint32_t (&c)[32], uint32_t sum_at) {
+  float sum = tmem_ld1(sum_at);
+#pragma unroll
+  for (int d = 0; d < 64; d += 32) {
+    if (d < D) {
+      float o[32];
+      tmem_ld32(o, acc + d);
+      tmem_wait_ld();
+      pin(o);
+      if (d == 0) pin(sum);
+#pragma unroll
+      for (int e = 0; e < 32; e += 16) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t x = c[(d + e) / 2 + i];
+          w[i] = Elem<T>::pack(fmaf(-sum, Elem<T>::lo(x), o[e + 2 * i]) * f,
+                               fmaf(-sum, Elem<T>::hi(x), o[e + 2 * i + 1]) * f);
+        }
+        if (out && d + e + 16 <= D)
+          store16(out + d + e, w);
+        else if (out && d + e < D)
+          *(uint4*)(out + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __syncwarp();  // tcgen05.ld takes the whole warp
+    }
   }
 }
 

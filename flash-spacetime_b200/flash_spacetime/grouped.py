@@ -18,7 +18,7 @@ Conventions:
 * with gradients, a 16-bit forward also keeps what rounding its output left
   over, so that the backward's row sums ``D = dO . out`` are those of the
   unrounded output: dq and dk would otherwise carry its rounding, times any
-  offset that the values share;
+  offset that the values share (an offset of the keys stays out of dq as well);
 * a row that sees one key (the row of an event of one, row 0 of a causal event)
   has a dq, and a share in dk, of exactly 0;
 * fp16 gradients keep their small values whatever the gradient's scale: dS
